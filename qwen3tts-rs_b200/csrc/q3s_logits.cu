@@ -676,26 +676,27 @@ __global__ void __launch_bounds__(T, ROWS == 2 ? 8 : 12) stream_kernel(const Log
 #pragma unroll 1
   for (; r < b.num_rows; r += gridDim.x) {
     const Meta m = next;
+    const int status = m.status(a);
+    const bool ok = status == Q3S_STATUS_OK;
     Row row;
     row.out = static_cast<char*>(b.out) + r * b.out_stride * width<OUT>;
     row.lo = row.first = 0;
     row.end = vocab;
     const Ids ids = row.take(a, m);
-    // On their way while the row is waited for and written out.
+    // On their way while the row is waited for and written out.  Of a refused row
+    // nothing is read: its ranges may lie anywhere.
     const bool last = rank >= T - 32;  // the warp of the biases
     RawIds raw;
     RawBias bias;
-    if (rank < ids.fours()) raw.load(ids.p, ids.type, ids.head + 4 * rank);
-    if (last && row.e0 + rank % 32 < row.e1) bias.load(b, row.e0 + rank % 32);
+    if (ok && rank < ids.fours()) raw.load(ids.p, ids.type, ids.head + 4 * rank);
+    if (ok && last && row.e0 + rank % 32 < row.e1) bias.load(b, row.e0 + rank % 32);
     if (!a.hold_refill) copy(r + (ROWS - 1ll) * gridDim.x, slot ? slot - 1 : ROWS - 1);
     const char* stage = ring + slot * a.stage;
     uint64_t* bar = &arrived[slot];
     const uint32_t phase = parity;
     if (++slot == ROWS) slot = 0, parity ^= 1;
     if (r + gridDim.x < b.num_rows) next = Meta(a, r + gridDim.x);
-    const int status = m.status(a);
     if (rank == 0) b.status[r] = (uint8_t)status;
-    const bool ok = status == Q3S_STATUS_OK;
     if (rank == 0) here[slot] = mbar_wait_bounded(bar, phase, a.wait_ns);
     sync();
     if (!here[slot]) break;

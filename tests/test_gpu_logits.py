@@ -553,3 +553,37 @@ def test_the_c_entry_refuses():
         assert "q3s_process_logits" in q3s.last_error()
     assert lib.q3s_process_logits(None, None, None) == q3s.E_INVALID_ARGUMENT
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("R", [20, 2000])
+def test_ranges_too_long_are_refused(R):
+    """A history or a bias list of 2^30 entries or more: UNSUPPORTED, the row
+    is left alone, and the rows around it are processed; the few-row and the
+    many-row kernel.  Every range starts on real entries; a refused row reads
+    none of them."""
+    V, n = 1024, 512
+    x = torch.randn((R, V), device=DEV)
+    hist = torch.randint(0, V, (n,), dtype=torch.int32, device=DEV)
+    offs = torch.zeros(R, dtype=torch.int64, device=DEV)
+    ends = offs + 40
+    ends[3::10] = 2 ** 30 + 8
+    ends[4::10] = 2 ** 62
+    bias_ids = torch.randint(0, V, (n,), dtype=torch.int32, device=DEV)
+    # A row whose list begins where the row before ended and ends far behind it.
+    boffs = torch.zeros(R + 1, dtype=torch.int64, device=DEV)
+    boffs[6::10] = 2 ** 31  # rows 5, 15, ... are too long; rows 6, 16, ... empty
+    pen = torch.tensor([1.3, 0.5, 0.25], device=DEV)
+    res = torch.full((R, V), 9.0, device=DEV)
+    st = torch.empty(R, dtype=torch.uint8, device=DEV)
+    q3s.process_logits(x, penalties=pen, history=hist, history_offsets=offs, history_ends=ends,
+                       bias_ids=bias_ids, bias_values=torch.ones(n, device=DEV), bias_offsets=boffs,
+                       out=(res, st))
+    bad = torch.zeros(R, dtype=torch.bool, device=DEV)
+    for k in (3, 4, 5):
+        bad[k::10] = True
+    assert torch.equal(st == q3s.STATUS_UNSUPPORTED, bad) and (st[~bad] == 0).all()
+    assert (res[bad] == 9.0).all()
+    good = x[~bad]
+    want, _ = q3s.process_logits(good, penalties=pen, history=hist,
+                                 history_offsets=offs[:len(good)], history_ends=ends[:1].repeat(len(good)))
+    assert torch.equal(res[~bad], want)
