@@ -281,9 +281,9 @@ int q3s_greedy_batch(q3s_context* ctx, const void* logits, int32_t dtype, int64_
  * A row whose parameters are invalid gets the status of the failure and -inf
  * in every entry, so that sampling it fails too: INVALID_REPETITION_PENALTY
  * (not finite or <= 0), INVALID_PENALTY, INVALID_MASK.  A row whose
- * row_vocab is negative or above vocab, or whose history or bias list holds
- * 2^30 entries or more, gets UNSUPPORTED and is not written.  vocab is at most
- * 2^26.
+ * row_vocab is negative or above vocab, whose history holds 2^30 ids or more,
+ * or whose bias list holds more than 2^20 entries, gets UNSUPPORTED and is not
+ * written.  vocab is at most 2^26.
  *
  * out may be logits itself, with its type and strides (INVALID_ARGUMENT
  * otherwise); it must not overlap logits in any other way.

@@ -46,6 +46,8 @@ constexpr int MAX_STREAM = 4096;     // entries of a row of the stream kernel
 constexpr int MAX_VOCAB = 1 << 26;
 
 constexpr int BIASES = 64;          // a chunk's bias entries that are kept at hand
+constexpr int WINDOW = 2 * BIASES;  // places whose sums take the same memory
+constexpr int MAX_BIASES = 1 << 20;  // of a row: 20 ms in one chunk, 81 ms in place
 
 // A counter word: the occurrences after the prompt, whether the prompt has the
 // id, and whether the bias list does.
@@ -55,6 +57,7 @@ constexpr uint32_t COUNT = BIASED - 1;
 
 struct LogitsArgs {
   q3s_logits_batch b;
+  long long row0;  // of the launch's first block
   int chunk;      // entries of a block
   int places;     // counters per chunk, a multiple of 8; 0 without histories
   int stage;      // bytes of the chunk's entries in shared memory
@@ -203,7 +206,7 @@ struct Meta {
     }
   }
   __device__ __forceinline__ int status(const LogitsArgs& a) const {
-    if (vocab < 0 || vocab > a.b.vocab || h1 - h0 > (long long)COUNT || e1 - e0 > (long long)COUNT)
+    if (vocab < 0 || vocab > a.b.vocab || h1 - h0 > (long long)COUNT || e1 - e0 > MAX_BIASES)
       return Q3S_STATUS_UNSUPPORTED;
     if (!isfinite(p.repetition) || p.repetition <= 0.0f) return Q3S_STATUS_INVALID_REPETITION_PENALTY;
     if (!isfinite(p.presence) || !isfinite(p.frequency)) return Q3S_STATUS_INVALID_PENALTY;
@@ -223,6 +226,20 @@ struct Row {
   double inverse;  // of the repetition penalty
   uint32_t ids, prompt;  // of the history, and how many of them are the prompt's
   long long e0, e1;      // biases
+
+  // Chunk `part` of row r.  Places start as far before the row as out's row starts
+  // behind a vector of VE: whole vectors of places are then aligned there.
+  template <int IN, int OUT, int VE>
+  static __device__ __forceinline__ Row part_of(const LogitsArgs& a, const Meta& m, long long r, int part) {
+    const q3s_logits_batch& b = a.b;
+    Row w;
+    w.in = static_cast<const char*>(b.logits) + (b.row_offsets ? m.offset : r * b.row_stride) * width<IN>;
+    w.out = static_cast<char*>(b.out) + (b.row_offsets ? m.offset : r * b.out_stride) * width<OUT>;
+    w.lo = part * a.chunk - (int)(reinterpret_cast<uintptr_t>(w.out) / width<OUT> % VE);
+    w.first = w.lo < 0 ? -w.lo : 0;
+    w.end = min(m.vocab - w.lo, a.chunk);
+    return w;
+  }
 
   // The rest from the metadata of a valid row; returns its history.
   __device__ __forceinline__ Ids take(const LogitsArgs& a, const Meta& m) {
@@ -313,10 +330,14 @@ __device__ __forceinline__ void count_ids(const Ids& ids, uint32_t prompt, uint3
   }
 }
 
-// The entries of the row's bias list that fall into the chunk, in list order.
-struct Biases {
-  uint32_t at[BIASES];
-  float value[BIASES];
+// The entries of the row's bias list that fall into the chunk, in list order, or
+// the sums of a window of places (add_many_biases).
+union Biases {
+  struct {
+    uint32_t at[BIASES];
+    float value[BIASES];
+  };
+  uint32_t sum[WINDOW];
 };
 
 // An entry as it lies in memory.
@@ -353,7 +374,7 @@ __device__ __forceinline__ int collect_biases(const q3s_logits_batch& b, const R
   return n;
 }
 
-// The same warp, a lane for each of the n entries get(i, at, value): the lane of
+// The same warp, a lane for each of the n entries of the list: the lane of
 // an id's first entry adds up its values in list order and writes the entry.
 // TAKE: the entry's counter is left at 0.  `held`: the lane's first entry's
 // logit and mask, already asked for.
@@ -368,47 +389,120 @@ __device__ __forceinline__ Held hold(const Row& row, uint32_t at) {
   return at == NOWHERE ? Held{0.0f, true} : Held{load_logit<IN>(row.in, i), masked(row, i)};
 }
 
-// The lane's first entry of what collect_biases() found.
-template <int IN>
-__device__ __forceinline__ Held hold_first(const q3s_logits_batch& b, const Row& row,
-                                           const Ids& ids, int given, const Biases& list) {
+// The place of the lane's first entry of the n that collect_biases() found.
+__device__ __forceinline__ uint32_t first_place(int n, const Biases& list) {
   const int lane = threadIdx.x % 32;
-  uint32_t at = NOWHERE;
-  if (given <= BIASES) {
-    if (lane < given) at = list.at[lane];
-  } else if (row.e0 + lane < row.e1) {
-    at = ids.place(__ldg(b.bias_ids + row.e0 + lane));
-  }
-  return hold<IN>(row, at);
+  return lane < n ? list.at[lane] : NOWHERE;
 }
 
-template <int IN, int OUT, bool TAKE, class Get>
+// Writes the entry at a place with the sum of its biases.
+template <int OUT, bool TAKE>
+__device__ __forceinline__ void write_biased(const Row& row, uint32_t* count, uint32_t at, Held held,
+                                             float sum) {
+  const uint32_t c = !row.ids ? 0 : TAKE ? atomicExch(count + at, 0u) : count[at];
+  if (!held.off)
+    store_logit<OUT>(row.out, row.lo + (int)at,
+                     __fadd_rn(c ? penalised(held.x, c, row.p, row.inverse) : held.x, sum));
+}
+
+template <int IN, int OUT, bool TAKE>
 __device__ __forceinline__ void add_biases(const Row& row, uint32_t* count, int n, Held held,
-                                           const Get& get) {
+                                           const Biases& list) {
   const int lane = threadIdx.x % 32;
   for (int e = lane; e < n; e += 32) {
-    uint32_t at;
-    float sum;
-    get(e, at, sum);
-    if (at == NOWHERE) continue;
-    const int i = row.lo + (int)at;
+    const uint32_t at = list.at[e];
+    float sum = list.value[e];
     if (e >= 32) held = hold<IN>(row, at);
-    const float x = held.x;
-    const bool off = held.off;
     bool first = true;
     for (int o = 0; o < n; ++o) {
-      uint32_t other;
-      float v;
-      get(o, other, v);
+      const uint32_t other = list.at[o];
+      const float v = list.value[o];  // asked for with the place, whether it counts or not
       if (other != at) continue;
       if (o < e) first = false;
       if (o > e) sum = __fadd_rn(sum, v);
     }
-    if (!first) continue;
-    const uint32_t c = !row.ids ? 0 : TAKE ? atomicExch(count + at, 0u) : count[at];
-    if (!off)
-      store_logit<OUT>(row.out, i,
-                       __fadd_rn(c ? penalised(x, c, row.p, row.inverse) : x, sum));
+    if (first) write_biased<OUT, TAKE>(row, count, at, held, sum);
+  }
+}
+
+// The same warp, where the chunk has more entries than `Biases` holds: the sums of a
+// window of places at a time, each in one walk over the row's list.  Looking each
+// entry's id up among all the others would take time in the square of the list;
+// this takes the list times the windows.  Lanes with one place take turns, so the
+// list order holds.  The sums lie where the chunk's entries did (`stage`, four bytes
+// a place), or where that is too small (in place there is none) in `list`: 300
+// biases on a row of 3072 f32 take 12 us in the one and 41 us in the other, 5000
+// 103 and 370 us.
+//
+// For chunk `part` of row r, from the batch alone and after all else in the kernel:
+// nothing has to live in registers until then.  (Called with the row in the middle of
+// stream_kernel, its loop spilled: 61440 rows of 2048 bf16 164 us instead of 126.)
+template <int IN, int OUT, int VE>
+__device__ __forceinline__ void add_many_biases(const LogitsArgs& a, long long r, int part,
+                                             uint32_t* count, Biases& list, char* stage,
+                                             int stage_bytes) {
+  constexpr int AHEAD = 4;
+  constexpr uint32_t NONE = 0xFFFFFFFFu;  // a NaN that no sum is left as
+  const int lane = threadIdx.x % 32;
+  const bool wide = stage_bytes >= 2 * (int)sizeof(Biases);
+  uint32_t* sum = wide ? reinterpret_cast<uint32_t*>(stage) : list.sum;
+  const int window = wide ? stage_bytes / 16 * 4 : WINDOW;
+  const q3s_logits_batch& b = a.b;
+  const Meta m(a, r);
+  Row row = Row::part_of<IN, OUT, VE>(a, m, r, part);
+  const Ids ids = row.take(a, m);
+  // Calls each(place in the window, value, whether there is one) for the list.
+  const auto walk = [&](int w0, const auto& each) {
+#pragma unroll 1
+    for (long long e = row.e0; e < row.e1; e += 32 * AHEAD) {
+      RawBias raw[AHEAD];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j)
+        if (e + j * 32 + lane < row.e1) raw[j].load(b, e + j * 32 + lane);
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        const uint32_t at = e + j * 32 + lane < row.e1 ? ids.place(raw[j].id) : NOWHERE;
+        const uint32_t to = at - (uint32_t)w0;
+        each(to, raw[j].value, at != NOWHERE && to < (uint32_t)window);
+      }
+    }
+  };
+  const auto write = [&](int w0, uint32_t to, uint32_t s) {
+    const uint32_t at = (uint32_t)w0 + to;
+    write_biased<OUT, false>(row, count, at, hold<IN>(row, at), __uint_as_float(s));
+  };
+  __syncwarp();
+#pragma unroll 1
+  for (int w0 = row.first; w0 < row.end; w0 += window) {
+    for (int j = 4 * lane; j < window; j += 128)
+      *reinterpret_cast<uint4*>(sum + j) = make_uint4(NONE, NONE, NONE, NONE);
+    __syncwarp();
+    walk(w0, [&](uint32_t to, float value, bool mine) {
+      if (!__any_sync(0xFFFFFFFFu, mine)) return;
+      const unsigned same = __match_any_sync(0xFFFFFFFFu, mine ? to : (uint32_t)window + lane);
+      const int turn = __popc(same & ((1u << lane) - 1));
+      for (int k = 0; __any_sync(0xFFFFFFFFu, mine && turn >= k); ++k) {
+        if (mine && turn == k) {
+          const uint32_t s = sum[to];
+          const float v = s == NONE ? value : __fadd_rn(__uint_as_float(s), value);
+          sum[to] = isnan(v) ? 0x7FFFFFFFu : __float_as_uint(v);
+        }
+        __syncwarp();
+      }
+    });
+    // Then each sum's entry: over the list once more, where who takes a sum writes
+    // its entry, or over the places, whichever are fewer.
+    if (row.e1 - row.e0 <= window) {
+      walk(w0, [&](uint32_t to, float, bool mine) {
+        const uint32_t s = mine ? atomicExch(sum + to, NONE) : NONE;
+        if (s != NONE) write(w0, to, s);
+      });
+    } else {
+#pragma unroll 4
+      for (int j = lane; j < window; j += 32)
+        if (sum[j] != NONE) write(w0, j, sum[j]);
+    }
+    __syncwarp();
   }
 }
 
@@ -456,9 +550,10 @@ __device__ __forceinline__ const char* copy_unlike(const Row& row, char* stage) 
 // The chunk in vectors of VE places, thread by thread side by side.  `stage`
 // holds the chunk's entries.  ALIKE: the rows of logits and out lie alike relative
 // to vectors of VE, and every thread reads back the vectors that it copied there;
-// else the places follow out's rows, and the entries are read one by one.
+// else the places follow out's rows, and the entries are read one by one.  Returns,
+// in the warp of the biases, whether they are still to be added (add_many_biases).
 template <int IN, int OUT, int VE, bool ALIKE>
-__device__ __forceinline__ void process(const LogitsArgs& a, const Row& row, const Ids& ids,
+__device__ __forceinline__ bool process(const LogitsArgs& a, const Row& row, const Ids& ids,
                                         uint32_t* count, char* stage, Biases& biases) {
   constexpr uint32_t ALL = (1u << VE) - 1;
   const q3s_logits_batch& b = a.b;
@@ -498,7 +593,7 @@ __device__ __forceinline__ void process(const LogitsArgs& a, const Row& row, con
   Held held{0.0f, true};
   if (row.e0 < row.e1 && last) {
     given = collect_biases(b, row, ids, count, biases, bias);
-    held = hold_first<IN>(b, row, ids, given, biases);
+    if (given <= BIASES) held = hold<IN>(row, first_place(given, biases));
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   if (row.ids || !ALIKE) __syncthreads();
@@ -572,52 +667,64 @@ __device__ __forceinline__ void process(const LogitsArgs& a, const Row& row, con
       }
     }
   }
-  if (row.e0 >= row.e1) return;
+  if (row.e0 >= row.e1) return false;
   __syncthreads();
-  if (given && given <= BIASES)
-    add_biases<IN, OUT, false>(row, count, given, held, [&](int i, uint32_t& at, float& v) {
-      at = biases.at[i];
-      v = biases.value[i];
-    });
-  else if (given)
-    add_biases<IN, OUT, false>(row, count, (int)(row.e1 - row.e0), held, [&](int i, uint32_t& at, float& v) {
-      at = ids.place(__ldg(b.bias_ids + row.e0 + i));
-      v = __ldg(b.bias_values + row.e0 + i);
-    });
+  if (given > BIASES) return true;
+  if (given) add_biases<IN, OUT, false>(row, count, given, held, biases);
+  return false;
 }
 
 template <int IN, int OUT, int VE, bool ALIKE>
-__global__ void __launch_bounds__(THREADS, BLOCKS) logits_kernel(const LogitsArgs a) {
+__global__ void __launch_bounds__(THREADS, BLOCKS) logits_kernel(
+    const __grid_constant__ LogitsArgs a) {
   static_assert(MAX_CHUNK / THREADS <= 64, "the mask bits of a thread fit two words");
   extern __shared__ uint4 smem[];
   __shared__ Biases biases;
   char* stage = reinterpret_cast<char*>(smem);
   uint32_t* count = reinterpret_cast<uint32_t*>(stage + a.stage);
   const q3s_logits_batch& b = a.b;
-  for (long long r = blockIdx.x; r < b.num_rows; r += gridDim.x) {
+  const long long r = a.row0 + blockIdx.x;
+  const Meta m(a, r);
+  const int status = m.status(a);
+  if (blockIdx.y == 0 && threadIdx.x == 0) b.status[r] = (uint8_t)status;
+  if (status == Q3S_STATUS_UNSUPPORTED) return;
+  Row row = Row::part_of<IN, OUT, VE>(a, m, r, blockIdx.y);
+  if (row.end <= row.first) return;
+  if (status != Q3S_STATUS_OK) {
+    for (int i = row.first + threadIdx.x; i < row.end; i += THREADS)
+      store_logit<OUT>(row.out, row.lo + i, neg_infinity());
+    return;
+  }
+  const Ids ids = row.take(a, m);
+  if (process<IN, OUT, VE, ALIKE>(a, row, ids, count, stage, biases))
+    add_many_biases<IN, OUT, VE>(a, r, blockIdx.y, count, biases, stage, a.stage);
+}
+
+// The rows of a block of stream_kernel whose bias lists hold more than `Biases`
+// does, after all its rows have been written without them: their entries once more,
+// from logits, with their counters counted again.  Apart from the loop, which has no
+// registers to spare; until then the row's status is that it has not run.
+template <int IN, int OUT, int VE, int T>
+__device__ __forceinline__ void add_long_lists(const LogitsArgs& a, uint32_t* count, Biases& biases,
+                                            char* ring, int ring_bytes) {
+  const int rank = threadIdx.x;
+#pragma unroll 1
+  for (long long r = blockIdx.x; r < a.b.num_rows; r += gridDim.x) {
     const Meta m(a, r);
-    const int status = m.status(a);
-    if (blockIdx.y == 0 && threadIdx.x == 0) b.status[r] = (uint8_t)status;
-    if (status == Q3S_STATUS_UNSUPPORTED) continue;
-    Row row;
-    row.in = static_cast<const char*>(b.logits) +
-             (b.row_offsets ? m.offset : r * b.row_stride) * width<IN>;
-    row.out = static_cast<char*>(b.out) +
-              (b.row_offsets ? m.offset : r * b.out_stride) * width<OUT>;
-    // Places start as far before the row as out's row starts behind a vector:
-    // whole vectors of places are then aligned there.
-    row.lo = (int)blockIdx.y * a.chunk - (int)(reinterpret_cast<uintptr_t>(row.out) / width<OUT> % VE);
-    row.first = row.lo < 0 ? -row.lo : 0;
-    row.end = min(m.vocab - row.lo, a.chunk);
-    if (row.end <= row.first) continue;
-    if (status != Q3S_STATUS_OK) {
-      for (int i = row.first + threadIdx.x; i < row.end; i += THREADS)
-        store_logit<OUT>(row.out, row.lo + i, neg_infinity());
-      continue;
-    }
+    if (m.status(a) != Q3S_STATUS_OK || m.e1 - m.e0 <= BIASES) continue;  // else done
+    Row row = Row::part_of<IN, OUT, VE>(a, m, r, 0);
     const Ids ids = row.take(a, m);
-    __syncthreads();  // the previous row's counters are no longer read
-    process<IN, OUT, VE, ALIKE>(a, row, ids, count, stage, biases);
+    RawIds raw;
+    if (rank < ids.fours()) raw.load(ids.p, ids.type, ids.head + 4 * rank);
+    if (row.ids) count_ids<T>(ids, row.prompt, count, raw);
+    __syncthreads();
+    if (rank >= T - 32) add_many_biases<IN, OUT, VE>(a, r, 0, count, biases, ring, ring_bytes);
+    if (rank == 0) a.b.status[r] = Q3S_STATUS_OK;
+    __syncthreads();
+    if (row.ids)
+      for (int i = 4 * rank; i < a.places; i += 4 * T)
+        *reinterpret_cast<uint4*>(count + i) = make_uint4(0, 0, 0, 0);
+    __syncthreads();
   }
 }
 
@@ -635,7 +742,8 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) logits_kernel(const LogitsArg
 // top and counted after the row is out, 129 / 308.  T = 64: 32 threads 137 / 371, 128
 // threads 160 / 319.
 template <int IN, int OUT, int VE, int ROWS, int T>
-__global__ void __launch_bounds__(T, ROWS == 2 ? 8 : 12) stream_kernel(const LogitsArgs a) {
+__global__ void __launch_bounds__(T, ROWS == 2 ? 6 : 12) stream_kernel(
+    const __grid_constant__ LogitsArgs a) {
   constexpr uint32_t ALL = (1u << VE) - 1;
   constexpr int AHEAD = 4;
   extern __shared__ uint4 smem[];
@@ -654,7 +762,9 @@ __global__ void __launch_bounds__(T, ROWS == 2 ? 8 : 12) stream_kernel(const Log
     *reinterpret_cast<uint4*>(count + i) = make_uint4(0, 0, 0, 0);
   __shared__ uint64_t arrived[ROWS];
   __shared__ int here[ROWS];  // one a row under way: a refused row ends without a barrier
+  __shared__ int late;  // rows whose bias lists are left to add_long_lists()
   if (rank == 0) {
+    late = 0;
     for (int s = 0; s < ROWS; ++s) mbar_init(&arrived[s], 1);
     fence_mbarrier_init();
   }
@@ -729,23 +839,17 @@ __global__ void __launch_bounds__(T, ROWS == 2 ? 8 : 12) stream_kernel(const Log
       }
     }
     int given = 0;  // known to the last warp
-    if (row.e0 < row.e1 && last) given = collect_biases(b, row, ids, count, biases, bias);
+    if (row.e0 < row.e1 && last)
+      given = row.e1 - row.e0 > BIASES ? BIASES + 1 : collect_biases(b, row, ids, count, biases, bias);
     if (row.ids) count_ids<T>(ids, row.prompt, count, raw);
     if (row.ids || row.e0 < row.e1) sync();
     row.in = stage;
-    Held held{0.0f, true};
-    if (given) held = hold_first<IN>(b, row, ids, given, biases);
-    if (given && given <= BIASES)
-      add_biases<IN, OUT, true>(row, count, given, held, [&](int i, uint32_t& at, float& v) {
-        at = biases.at[i];
-        v = biases.value[i];
-      });
-    else if (given)
-      add_biases<IN, OUT, true>(row, count, (int)(row.e1 - row.e0), held,
-                                [&](int i, uint32_t& at, float& v) {
-                                  at = ids.place(__ldg(b.bias_ids + row.e0 + i));
-                                  v = __ldg(b.bias_values + row.e0 + i);
-                                });
+    if (given > BIASES) {
+      if (rank % 32 == 0) b.status[r] = Q3S_STATUS_NOT_RUN, late = 1;
+    } else if (given) {
+      const Held held = hold<IN>(row, first_place(given, biases));
+      add_biases<IN, OUT, true>(row, count, given, held, biases);
+    }
     if (row.ids) {
       // Who takes an entry's counter writes the entry; the biases took theirs.
       const auto write = [&](uint4 places) {
@@ -756,11 +860,34 @@ __global__ void __launch_bounds__(T, ROWS == 2 ? 8 : 12) stream_kernel(const Log
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           c[e] = c[e] && !(c[e] & BIASED) ? atomicExch(count + at[e], 0u) : 0;
+        if (ROWS == 2) {
+          // Side by side, so that their latencies overlap (65536 rows of 3072 f32 274 us, one
+          // after the other 289 us); with four rows in the ring there are no registers for
+          // that (61440 rows of 2048 bf16 141 us, 127 us this way).
+          float x[4], q[4];
+          bool divide = false;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (c[e] && !masked(row, (int)at[e]))
-            store_logit<OUT>(row.out, at[e],
-                             penalised(load_logit<IN>(stage, at[e]), c[e], row.p, row.inverse));
+          for (int e = 0; e < 4; ++e) x[e] = c[e] ? load_logit<IN>(stage, at[e]) : 0.0f;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            q[e] = quotient(x[e], row.inverse);
+            divide = divide || subnormal(x[e], q[e]);
+          }
+          if (divide) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[e] = __fdiv_rn(x[e], row.p.repetition);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (c[e] && !masked(row, (int)at[e]))
+              store_logit<OUT>(row.out, at[e], penalised_by(x[e], c[e], row.p, q[e]));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (c[e] && !masked(row, (int)at[e]))
+              store_logit<OUT>(row.out, at[e],
+                               penalised(load_logit<IN>(stage, at[e]), c[e], row.p, row.inverse));
+        }
       };
       const uint32_t fours = ids.fours(), rest = ids.n - 4 * fours;
       if (rank < rest)
@@ -774,7 +901,10 @@ __global__ void __launch_bounds__(T, ROWS == 2 ? 8 : 12) stream_kernel(const Log
     }
     sync();  // the row and the counters are no longer read
   }
-  if (r >= b.num_rows) return;
+  if (r >= b.num_rows) {
+    if (late) add_long_lists<IN, OUT, VE, T>(a, count, biases, ring, ROWS * a.stage);
+    return;
+  }
   // A copy did not come in time: its row and those after it have not run.  The
   // block stays, for a limited time, until no copy is under way to its ring.
   if (rank == 0) {
@@ -815,15 +945,20 @@ cudaError_t launch(LogitsArgs& a, bool aligned, const ContextInfo& ci, cudaStrea
   const cudaError_t e = allow_smem((const void*)logits_kernel<IN, OUT, VE, ALIKE>,
                                    MAX_CHUNK * (width<IN> + 4) + 16, ci.device, allowed);
   if (e != cudaSuccess) return e;
-  const dim3 grid((unsigned)(a.b.num_rows < 0x7FFFFFFF ? a.b.num_rows : 0x7FFFFFFF),
-                  (unsigned)chunks(a.chunk));
-  logits_kernel<IN, OUT, VE, ALIKE><<<grid, THREADS, a.stage + a.places * 4, st>>>(a);
-  return cudaGetLastError();
+  for (a.row0 = 0; a.row0 < a.b.num_rows; a.row0 += 0x7FFFFFFF) {  // as many as a grid can have
+    const long long rows = a.b.num_rows - a.row0;
+    const dim3 grid((unsigned)(rows < 0x7FFFFFFF ? rows : 0x7FFFFFFF), (unsigned)chunks(a.chunk));
+    logits_kernel<IN, OUT, VE, ALIKE><<<grid, THREADS, a.stage + a.places * 4, st>>>(a);
+    const cudaError_t l = cudaGetLastError();
+    if (l != cudaSuccess) return l;
+  }
+  return cudaSuccess;
 }
 
 template <int IN, int OUT, int VE, int ROWS, int T>
 cudaError_t launch_stream(LogitsArgs& a, const ContextInfo& ci, cudaStream_t st) {
   a.stage = a.b.vocab * width<IN>;
+  a.chunk = a.b.vocab;
   if (a.b.params && a.b.history_offsets) a.places = a.b.vocab;
   const int smem = ROWS * a.stage + a.places * 4;
   static std::atomic<uint64_t> allowed{0};
@@ -851,9 +986,10 @@ cudaError_t launch_typed(LogitsArgs& a, const ContextInfo& ci, cudaStream_t st) 
                      (one || b.row_offsets || (b.row_stride - b.out_stride) % VE == 0);
   const bool aligned = in % VE == 0 && (one || (!b.row_offsets && b.row_stride % VE == 0));
   // Eight rows a multiprocessor, of one length, that start on 16 bytes.  Two rows of
-  // 8192 bytes or more in the ring (eight blocks a multiprocessor; twelve spill
-  // registers, 442 us against 308 for 65536 rows of 3072 f32), four of shorter ones
-  // (twelve blocks: 123 us for 61440 rows of 2048 bf16, 128 us with ten).
+  // 8192 bytes or more in the ring (registers for six blocks a multiprocessor at
+  // least; twelve spill, 442 us against 308 for 65536 rows of 3072 f32 at that step),
+  // four of shorter ones (twelve blocks: 123 us for 61440 rows of 2048 bf16, 128 us
+  // with ten).
   const int stage = b.vocab * width<IN>;
   if (b.num_rows >= 8LL * ci.sm_count && !b.row_offsets && !b.row_vocab && !a.in_place && alike &&
       b.vocab > 0 && b.vocab <= MAX_STREAM && b.vocab % 8 == 0 &&

@@ -1287,8 +1287,8 @@ def process_logits(logits, *, penalties=None, history=None, history_offsets=None
     history_offsets[r + 1]), or up to history_ends[r]; the first
     prompt_lens[r] of them count for the repetition penalty only.
     bias_ids (int32) and bias_values (float32): row r's entries are
-    [bias_offsets[r], bias_offsets[r + 1]) (int64 [R + 1]); repeated ids add
-    up.  masks: int32 [M, words] of allowed bits (pack_mask); row r uses mask
+    [bias_offsets[r], bias_offsets[r + 1]) (int64 [R + 1], at most 2^20 a
+    row); repeated ids add up.  masks: int32 [M, words] of allowed bits (pack_mask); row r uses mask
     mask_rows[r] (int32, negative: none), or mask r without mask_rows.
     Returns (out, status uint8 [R]); out has out_dtype (the logits' by
     default), and may be given as out=(tensor, status), the logits included.

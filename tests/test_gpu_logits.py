@@ -587,3 +587,103 @@ def test_ranges_too_long_are_refused(R):
     want, _ = q3s.process_logits(good, penalties=pen, history=hist,
                                  history_offsets=offs[:len(good)], history_ends=ends[:1].repeat(len(good)))
     assert torch.equal(res[~bad], want)
+
+
+def _bias_args(lists):
+    """Lists of (ids, values) as the arguments of process_logits."""
+    offs = np.concatenate([[0], np.cumsum([len(i) for i, _ in lists])])
+    return dict(
+        bias_ids=torch.from_numpy(np.concatenate([i for i, _ in lists])).to(torch.int32).to(DEV),
+        bias_values=torch.from_numpy(np.concatenate([v for _, v in lists]).astype(np.float32)).to(DEV),
+        bias_offsets=torch.from_numpy(offs).to(DEV))
+
+
+def _list_sums(V, ids, values):
+    """(sums, which ids have one): every id's values added in f32, in list order."""
+    want, has = np.zeros(V, np.float32), np.zeros(V, bool)
+    for i, v in zip(ids, values.astype(np.float32)):
+        want[i] = want[i] + v if has[i] else v
+        has[i] = True
+    return want, has
+
+
+@pytest.mark.parametrize("dtype,out", [("f32", "f32"), ("bf16", "bf16"), ("bf16", "f32")])
+@pytest.mark.parametrize("R,V,bias", [(3, 700, 300), (5, 9001, 3000), (1500, 520, 90),
+                                      (1300, 3072, 400)])
+def test_more_biases_than_a_block_keeps_at_hand(R, V, bias, dtype, out):
+    """Lists that overflow a block's own, with histories and masks, in the
+    few-row and the many-row kernel; out of place and in place."""
+    c = Case(R + V + bias, R, V, dtype, out, hist=60, bias=bias, masks=3)
+    got, st = run(c)
+    rows = np.unique(np.concatenate([np.arange(min(R, 12)), np.arange(max(0, R - 12), R)]))
+    sub = dict(c.oracle)
+    for k in ("histories", "biases", "allowed"):
+        sub[k] = [sub[k][r] for r in rows]
+    for k in ("penalties", "prompt_lens"):
+        sub[k] = sub[k][rows]
+    value, bound = so.process_logits(c.x[rows], **sub)
+    so.check(got[torch.from_numpy(rows).to(DEV)].double().cpu().numpy(), value,
+             so.rounded(bound, value, out == "bf16"))
+    assert (st == 0).all()
+    if dtype == out:  # in place runs in the few-row kernel
+        q3s.process_logits(c.logits, **c.args, out=(c.logits, st))
+        assert torch.equal(c.logits, got) and (st == 0).all()
+
+
+@pytest.mark.parametrize("R,V,n", [(1, 100, 150), (2, 3000, 5000), (1200, 64, 200), (1200, 2048, 1000)])
+def test_long_bias_lists_add_up_in_list_order(R, V, n):
+    """Bit for bit, with values whose f32 sum depends on the order: ids that
+    repeat side by side, within 32 entries and far apart."""
+    rng = np.random.default_rng(n)
+    lists = []
+    for r in range(R):
+        ids = rng.integers(0, V, n)
+        ids[: n // 3] = rng.integers(0, 5, n // 3)
+        ids[n // 2: n // 2 + 40] = V - 1
+        values = rng.standard_normal(n) * 10.0 ** rng.integers(-4, 5, n)
+        lists.append((ids, values.astype(np.float32)))
+    x = torch.zeros((R, V), device=DEV)
+    out, st = q3s.process_logits(x, **_bias_args(lists))
+    out = out.cpu().numpy()
+    for r in {0, R // 2, R - 1}:
+        np.testing.assert_array_equal(out[r], _list_sums(V, *lists[r])[0])
+    assert (st == 0).all()
+
+
+@pytest.mark.parametrize("R", [2, 1200])
+def test_special_values_in_long_bias_lists(R):
+    """Infinities that cancel, NaN of any payload and a NaN before a number:
+    NaN in those entries, and only there."""
+    V, n = 256, 200
+    ids = np.arange(n) % 150
+    bits = np.float32(1.0).view(np.uint32) + np.zeros(n, np.uint32)
+    values = bits.view(np.float32)
+    bits[7], bits[9], bits[160] = 0xFFFFFFFF, 0x7FC00001, 0xFFFFFFFF  # id 10 comes at 10 and 160
+    values[3], values[153] = np.inf, -np.inf                          # id 3 twice
+    values[20] = -np.inf
+    x = torch.zeros((R, V), device=DEV)
+    out, _ = q3s.process_logits(x, **_bias_args([(ids, values)] * R))
+    want = np.zeros(V, np.float32)
+    with np.errstate(invalid="ignore"):
+        np.add.at(want, ids, values)
+    assert np.isnan(want).nonzero()[0].tolist() == [3, 7, 9, 10]
+    for r in (0, R - 1):
+        np.testing.assert_array_equal(out[r].cpu().numpy(), want)
+
+
+def test_the_longest_bias_list():
+    """2^20 entries are added up; one more is refused, and the row left alone."""
+    V, n = 700, 2 ** 20
+    ids = torch.randint(0, V, (n + 1,), device=DEV).to(torch.int32)
+    one = torch.ones(n + 1, device=DEV)
+    x = torch.zeros((2, V), device=DEV)
+    res, st = torch.full((2, V), 9.0, device=DEV), torch.empty(2, dtype=torch.uint8, device=DEV)
+    q3s.process_logits(x, bias_ids=ids, bias_values=one, out=(res, st),
+                       bias_offsets=torch.tensor([0, n, n], device=DEV))
+    want = torch.bincount(ids[:n].long(), minlength=V).float()
+    assert torch.equal(res[0], want) and torch.equal(res[1], x[1]) and st.tolist() == [0, 0]
+    res.fill_(9.0)
+    q3s.process_logits(x, bias_ids=ids, bias_values=one, out=(res, st),
+                       bias_offsets=torch.tensor([0, n + 1, n + 1], device=DEV))
+    assert st.tolist() == [q3s.STATUS_UNSUPPORTED, 0]
+    assert (res[0] == 9.0).all() and torch.equal(res[1], x[1])
