@@ -370,7 +370,7 @@ int q3s_embed_lookup(q3s_context* ctx, const q3s_lookup_batch* batch, void* stre
  * the valid rows for a broadcast one (text_stride 0); it has grads_dtype, is
  * not scaled and not accumulated.  The workspace belongs to the context and
  * the stream and grows on demand: before capturing a call into a graph, make
- * it once. */
+ * it once.  Calls of several host threads may share a context and a stream. */
 typedef struct q3s_embed_grad_batch {
   int32_t dtype;       /* Q3S_DTYPE_* of grad_out */
   int32_t grads_dtype; /* Q3S_DTYPE_* of grads and text_grad */

@@ -4,6 +4,7 @@
 #include <cmath>
 #include <cstdio>
 #include <cstring>
+#include <memory>
 #include <mutex>
 #include <string>
 #include <vector>
@@ -88,15 +89,22 @@ struct q3s_context {
   };
   std::mutex ws_mu;
   std::vector<Workspace> ws;
-  // Workspaces of the embedding gradient (stream_scratch), one per stream,
-  // and the outgrown ones, which captured graphs may still use.
+  // Workspaces of the embedding gradient (stream_scratch), one per stream, each
+  // with the outgrown ones, which captured graphs may still use.
   struct Scratch {
     cudaStream_t stream;
-    unsigned char* ptr;
-    size_t bytes;
+    unsigned char* ptr = nullptr;
+    size_t bytes = 0;
+    std::vector<unsigned char*> outgrown;
+    std::mutex busy;  // held while a call's kernels are launched
+
+    explicit Scratch(cudaStream_t s) : stream(s) {}
+    ~Scratch() {
+      if (ptr) cudaFree(ptr);
+      for (auto* p : outgrown) cudaFree(p);
+    }
   };
-  std::vector<Scratch> scratch;
-  std::vector<unsigned char*> outgrown;
+  std::vector<std::unique_ptr<Scratch>> scratch;
   // Testing hooks (q3s_context_set_test_hooks).
   uint64_t test_wait_ns = 0;
   int test_hold_refill = 0;
@@ -123,23 +131,27 @@ int record_error(int code, const std::string& msg) { return fail(code, msg); }
 
 int record_cuda_error(cudaError_t e, const char* what) { return cuda_fail(e, what); }
 
-int stream_scratch(q3s_context* ctx, void* stream, size_t need, unsigned char** scratch) {
-  std::lock_guard<std::mutex> lock(ctx->ws_mu);
+int stream_scratch(q3s_context* ctx, void* stream, size_t need, unsigned char** scratch,
+                   std::unique_lock<std::mutex>* busy) {
   const cudaStream_t key = (cudaStream_t)stream;
   q3s_context::Scratch* w = nullptr;
-  for (auto& x : ctx->scratch)
-    if (x.stream == key) w = &x;
-  if (!w) {
-    ctx->scratch.push_back(q3s_context::Scratch{key, nullptr, 0});
-    w = &ctx->scratch.back();
+  {
+    std::lock_guard<std::mutex> lock(ctx->ws_mu);
+    for (auto& x : ctx->scratch)
+      if (x->stream == key) w = x.get();
+    if (!w) {
+      ctx->scratch.push_back(std::make_unique<q3s_context::Scratch>(key));
+      w = ctx->scratch.back().get();
+    }
   }
+  *busy = std::unique_lock<std::mutex>(w->busy);
   if (need > w->bytes) {
     // At least doubled, so that the outgrown ones together stay below the last.
     const size_t bytes = need > 2 * w->bytes ? need : 2 * w->bytes;
     unsigned char* p = nullptr;
     const cudaError_t e = cudaMalloc((void**)&p, bytes);
     if (e != cudaSuccess) return cuda_fail(e, "cudaMalloc(workspace)");
-    if (w->ptr) ctx->outgrown.push_back(w->ptr);
+    if (w->ptr) w->outgrown.push_back(w->ptr);
     w->ptr = p;
     w->bytes = bytes;
   }
@@ -225,9 +237,7 @@ void q3s_context_destroy(q3s_context* c) {
       if (w.ptr) cudaFree(w.ptr);
       if (w.counter) cudaFree(w.counter);
     }
-    for (auto& w : c->scratch)
-      if (w.ptr) cudaFree(w.ptr);
-    for (auto* p : c->outgrown) cudaFree(p);
+    c->scratch.clear();
   }
   delete c;
 }

@@ -18,6 +18,7 @@
 // is read once for each group; the groups' reads of rows that are still in L2
 // count against L2.  Each kernel starts while the one before it ends.
 #include <cstdint>
+#include <mutex>
 #include <string>
 #include <type_traits>
 
@@ -938,7 +939,8 @@ int embed_grad(q3s_context* ctx, const q3s_embed_grad_batch* b, void* stream) {
     need += list * (groups > 1 ? 2 : 1) + align256((size_t)a.vocab[g] * sizeof(uint2)) + partial;
   need += align256((size_t)groups * 4);
   unsigned char* p = nullptr;
-  rc = stream_scratch(ctx, stream, need, &p);
+  std::unique_lock<std::mutex> busy;
+  rc = stream_scratch(ctx, stream, need, &p, &busy);
   if (rc != Q3S_OK) return rc;
   for (int g = 0; g < groups; ++g) {
     a.work[g].rows = reinterpret_cast<uint32_t*>(p);

@@ -5,6 +5,7 @@
 #include <atomic>
 #include <cstddef>
 #include <cstdint>
+#include <mutex>
 #include <string>
 
 #include <cuda_runtime.h>
@@ -31,10 +32,13 @@ int record_error(int code, const std::string& msg);
 int record_cuda_error(cudaError_t e, const char* what);
 
 // A device workspace of at least `need` bytes that belongs to the context and
-// the stream: launches on one stream are ordered, so they share it.  It grows
-// on demand; an outgrown one lives until the context is destroyed, because a
-// captured graph may still use it.  Its contents are undefined.
-int stream_scratch(q3s_context* ctx, void* stream, size_t need, unsigned char** scratch);
+// the stream: launches on one stream are ordered, so they share it.  Those of one
+// call must follow one another, whatever thread launches on the stream too: `busy`
+// is locked for that and has to stay so until the call's last launch.  The
+// workspace grows on demand; an outgrown one lives until the context is destroyed,
+// because a captured graph may still use it.  Its contents are undefined.
+int stream_scratch(q3s_context* ctx, void* stream, size_t need, unsigned char** scratch,
+                   std::unique_lock<std::mutex>* busy);
 
 // Makes `device` current for the scope and restores the caller's device.
 struct DeviceScope {

@@ -24,6 +24,7 @@ from __future__ import annotations
 import ctypes
 import os
 import struct
+import threading
 from dataclasses import dataclass
 from pathlib import Path
 from typing import Callable, Optional, Sequence
@@ -399,6 +400,7 @@ class Context:
 
 
 _default_ctx: dict = {}
+_default_ctx_lock = threading.Lock()
 
 
 def default_context(device: Optional[int] = None) -> Context:
@@ -406,8 +408,9 @@ def default_context(device: Optional[int] = None) -> Context:
         return _default_ctx[device]
     import torch
     d = torch.cuda.current_device() if device is None else int(device)
-    if d not in _default_ctx:
-        _default_ctx[d] = Context(d)
+    with _default_ctx_lock:  # one context, whichever thread asks first
+        if d not in _default_ctx:
+            _default_ctx[d] = Context(d)
     return _default_ctx[d]
 
 

@@ -378,3 +378,48 @@ def test_the_c_entry_refuses():
         assert "q3s_embed_grad" in q3s.last_error()
     assert lib.q3s_embed_grad(None, None, None) == q3s.E_INVALID_ARGUMENT
     torch.cuda.synchronize()
+
+
+def test_threads_on_one_stream():
+    """Calls of several host threads on one stream, through the context they
+    share: the launches of a call stay together, so each gets its own sums."""
+    import threading
+    rng = np.random.default_rng(10)
+    jobs = []
+    for R, vocabs, H in ((3000, [700, 300, 40], 64), (257, [50, 60], 32), (9000, [900], 16),
+                         (1200, [40] * 9, 128)):
+        codes = torch.from_numpy(_codes(rng, R, vocabs, 2.0)).to(DEV)
+        grad = _grad(rng, R, H, "f32")
+        jobs.append((codes, grad, vocabs, q3s.embed_sum_grad(codes, grad, vocabs)))
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    start, wrong = threading.Barrier(len(jobs)), []
+
+    def work(codes, grad, vocabs, want):
+        start.wait()
+        for _ in range(100):
+            with torch.cuda.stream(stream):
+                got = q3s.embed_sum_grad(codes, grad, vocabs)
+                if not all(torch.equal(a, b) for a, b in zip(got, want)):
+                    wrong.append(len(codes))
+
+    threads = [threading.Thread(target=work, args=j) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_threads_get_one_default_context():
+    import threading
+    from unittest import mock
+    got = []
+    with mock.patch.dict(q3s._default_ctx, clear=True):
+        threads = [threading.Thread(target=lambda: got.append(q3s.default_context(0)))
+                   for _ in range(8)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert len(got) == 8 and all(c is got[0] for c in got)
