@@ -368,9 +368,14 @@ int q3s_embed_lookup(q3s_context* ctx, const q3s_lookup_batch* batch, void* stre
  * identity.  text_grad (optional) is the gradient of its text operand:
  * grad_out on valid rows and zero elsewhere for a text per row, the sum over
  * the valid rows for a broadcast one (text_stride 0); it has grads_dtype, is
- * not scaled and not accumulated.  The workspace belongs to the context and
- * the stream and grows on demand: before capturing a call into a graph, make
- * it once.  Calls of several host threads may share a context and a stream. */
+ * not scaled and not accumulated.
+ *
+ * The workspace belongs to the context and grows on demand.  Direct calls on
+ * one stream share one; a captured call has one of its own, so that replays may
+ * run beside direct calls and other graphs (but not two instantiations of one
+ * graph beside each other).  It is kept until the graph is destroyed, which must
+ * not be before its last replay has ended, and the context has to outlive both.
+ * Calls of several host threads may share a context and a stream. */
 typedef struct q3s_embed_grad_batch {
   int32_t dtype;       /* Q3S_DTYPE_* of grad_out */
   int32_t grads_dtype; /* Q3S_DTYPE_* of grads and text_grad */

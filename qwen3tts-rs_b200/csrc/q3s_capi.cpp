@@ -1,6 +1,7 @@
 // C ABI of the B200 sampler (include/q3s_sampler.h): contexts, the batched
 // launch, the greedy launch and the stateful `Sampler` mirror of
 // src/talker/sampling.rs:144-335.
+#include <atomic>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
@@ -89,19 +90,21 @@ struct q3s_context {
   };
   std::mutex ws_mu;
   std::vector<Workspace> ws;
-  // Workspaces of the embedding gradient (stream_scratch), one per stream, each
-  // with the outgrown ones, which captured graphs may still use.
+  // Workspaces of the embedding gradient (stream_scratch): one per stream for
+  // direct calls, and one per stream of a capture for the graph that comes of it.
   struct Scratch {
     cudaStream_t stream;
     unsigned char* ptr = nullptr;
     size_t bytes = 0;
-    std::vector<unsigned char*> outgrown;
     std::mutex busy;  // held while a call's kernels are launched
+    // Of a capture (else NULL): whether its graph, or what was made of it, still
+    // exists.
+    std::shared_ptr<std::atomic<bool>> used;
+    unsigned long long capture = 0;  // its id
 
     explicit Scratch(cudaStream_t s) : stream(s) {}
     ~Scratch() {
       if (ptr) cudaFree(ptr);
-      for (auto* p : outgrown) cudaFree(p);
     }
   };
   std::vector<std::unique_ptr<Scratch>> scratch;
@@ -131,28 +134,117 @@ int record_error(int code, const std::string& msg) { return fail(code, msg); }
 
 int record_cuda_error(cudaError_t e, const char* what) { return cuda_fail(e, what); }
 
+namespace {
+
+using Used = std::shared_ptr<std::atomic<bool>>;
+
+// The destructor of the object that a captured graph holds.  It may run on a
+// thread of the driver's and after the context is gone, and calls nothing.
+void CUDART_CB graph_is_gone(void* p) {
+  Used* used = static_cast<Used*>(p);
+  (*used)->store(false);
+  delete used;
+}
+
+// Clears `used` when the graph and all that is instantiated from it are destroyed.
+cudaError_t clear_with_graph(cudaGraph_t graph, const Used& used) {
+  cudaUserObject_t object;
+  Used* held = new Used(used);
+  cudaError_t e = cudaUserObjectCreate(&object, held, graph_is_gone, 1, cudaUserObjectNoDestructorSync);
+  if (e != cudaSuccess) {
+    delete held;
+    return e;
+  }
+  e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
+  if (e != cudaSuccess) cudaUserObjectRelease(object, 1);
+  return e;
+}
+
+// cudaMalloc, which a capture in the strict modes forbids to its thread although it
+// adds nothing to the graph.
+cudaError_t malloc_in_capture(unsigned char** p, size_t bytes) {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) return e;
+  e = cudaMalloc((void**)p, bytes);
+  const cudaError_t back = cudaThreadExchangeStreamCaptureMode(&mode);
+  return e == cudaSuccess ? back : e;
+}
+
+// The workspace of a call that is captured: this capture's on this stream if it is
+// large enough, else one whose graph is gone, else a new one.
+int capture_scratch(q3s_context* ctx, cudaStream_t key, unsigned long long id, cudaGraph_t graph,
+                    size_t need, q3s_context::Scratch** out) {
+  q3s_context::Scratch* w = nullptr;
+  for (auto& x : ctx->scratch)
+    if (x->used && x->used->load() && x->capture == id && x->stream == key && x->bytes >= need)
+      w = x.get();
+  *out = w;
+  if (w) return Q3S_OK;
+  for (auto& x : ctx->scratch)
+    if (x->used && !x->used->load() && x->bytes >= need && (!w || x->bytes < w->bytes)) w = x.get();
+  if (!w) {
+    auto fresh = std::make_unique<q3s_context::Scratch>(key);
+    fresh->used = std::make_shared<std::atomic<bool>>(false);
+    const cudaError_t e = malloc_in_capture(&fresh->ptr, need);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaMalloc(workspace)");
+    fresh->bytes = need;
+    ctx->scratch.push_back(std::move(fresh));
+    w = ctx->scratch.back().get();
+  }
+  w->used->store(true);
+  w->stream = key;
+  w->capture = id;
+  const cudaError_t e = clear_with_graph(graph, w->used);
+  if (e != cudaSuccess) {
+    w->used->store(false);
+    return cuda_fail(e, "cudaGraphRetainUserObject");
+  }
+  *out = w;
+  return Q3S_OK;
+}
+
+}  // namespace
+
 int stream_scratch(q3s_context* ctx, void* stream, size_t need, unsigned char** scratch,
                    std::unique_lock<std::mutex>* busy) {
   const cudaStream_t key = (cudaStream_t)stream;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  cudaGraph_t graph = nullptr;
+  cudaError_t e = cudaSuccess;
+  // The legacy stream is never captured.
+  if (key && key != cudaStreamLegacy) e = cudaStreamIsCapturing(key, &status);
+  const bool captured = status == cudaStreamCaptureStatusActive;
+  if (e == cudaSuccess && captured) e = cudaStreamGetCaptureInfo(key, &status, &id, &graph);
+  if (e == cudaSuccess && status == cudaStreamCaptureStatusInvalidated)
+    e = cudaErrorStreamCaptureInvalidated;
+  if (e != cudaSuccess) return cuda_fail(e, "cudaStreamGetCaptureInfo");
   q3s_context::Scratch* w = nullptr;
   {
     std::lock_guard<std::mutex> lock(ctx->ws_mu);
-    for (auto& x : ctx->scratch)
-      if (x->stream == key) w = x.get();
-    if (!w) {
-      ctx->scratch.push_back(std::make_unique<q3s_context::Scratch>(key));
-      w = ctx->scratch.back().get();
+    if (captured) {
+      const int rc = capture_scratch(ctx, key, id, graph, need, &w);
+      if (rc != Q3S_OK) return rc;
+    } else {
+      for (auto& x : ctx->scratch)
+        if (x->stream == key && !x->used) w = x.get();
+      if (!w) {
+        ctx->scratch.push_back(std::make_unique<q3s_context::Scratch>(key));
+        w = ctx->scratch.back().get();
+      }
     }
   }
   *busy = std::unique_lock<std::mutex>(w->busy);
   if (need > w->bytes) {
-    // At least doubled, so that the outgrown ones together stay below the last.
-    const size_t bytes = need > 2 * w->bytes ? need : 2 * w->bytes;
-    unsigned char* p = nullptr;
-    const cudaError_t e = cudaMalloc((void**)&p, bytes);
+    // Half as much again at least, so that slowly growing calls seldom come here.
+    const size_t bytes = need > w->bytes + w->bytes / 2 ? need : w->bytes + w->bytes / 2;
+    // cudaFree waits for the device, so no launch still uses the old one.
+    if (w->ptr) cudaFree(w->ptr);
+    w->ptr = nullptr;
+    w->bytes = 0;
+    e = cudaMalloc((void**)&w->ptr, bytes);
     if (e != cudaSuccess) return cuda_fail(e, "cudaMalloc(workspace)");
-    if (w->ptr) w->outgrown.push_back(w->ptr);
-    w->ptr = p;
     w->bytes = bytes;
   }
   *scratch = w->ptr;

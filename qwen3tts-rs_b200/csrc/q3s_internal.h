@@ -34,9 +34,10 @@ int record_cuda_error(cudaError_t e, const char* what);
 // A device workspace of at least `need` bytes that belongs to the context and
 // the stream: launches on one stream are ordered, so they share it.  Those of one
 // call must follow one another, whatever thread launches on the stream too: `busy`
-// is locked for that and has to stay so until the call's last launch.  The
-// workspace grows on demand; an outgrown one lives until the context is destroyed,
-// because a captured graph may still use it.  Its contents are undefined.
+// is locked for that and has to stay so until the call's last launch.  It
+// grows on demand.  Calls that are captured get a workspace of their own, which no
+// other call is given while the graph or anything instantiated from it exists: a
+// replay may run beside direct calls and other graphs.  Its contents are undefined.
 int stream_scratch(q3s_context* ctx, void* stream, size_t need, unsigned char** scratch,
                    std::unique_lock<std::mutex>* busy);
 

@@ -423,3 +423,94 @@ def test_threads_get_one_default_context():
         for t in threads:
             t.join()
         assert len(got) == 8 and all(c is got[0] for c in got)
+
+
+def _captured(codes, grad, vocabs, stream, ctx=None):
+    """(the graph of one call captured on `stream`, its outputs)."""
+    out = [torch.empty((v, grad.shape[1]), device=DEV) for v in vocabs]
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=stream):
+        q3s.embed_sum_grad(codes, grad, vocabs, out=out, ctx=ctx)
+    return g, out
+
+
+def test_graphs_and_direct_calls_run_side_by_side():
+    """Two graphs captured on one stream, replayed on two others while direct
+    calls run on the capture stream: each has a workspace of its own."""
+    rng = np.random.default_rng(11)
+    capture, streams = torch.cuda.Stream(), [torch.cuda.Stream() for _ in range(2)]
+    jobs = []
+    for R, vocabs, H in ((9000, [900, 30], 64), (1500, [700, 300, 40], 128), (4000, [50, 60], 32)):
+        codes = torch.from_numpy(_codes(rng, R, vocabs, 2.0)).to(DEV)
+        grad = _grad(rng, R, H, "f32")
+        jobs.append((codes, grad, vocabs, q3s.embed_sum_grad(codes, grad, vocabs)))
+    graphs = [_captured(*j[:3], capture) for j in jobs[:2]]
+    wrong = []
+    for _ in range(30):
+        for s, (g, out) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                for t in out:
+                    t.zero_()
+                for _ in range(5):
+                    g.replay()
+        with torch.cuda.stream(capture):
+            got = [q3s.embed_sum_grad(*jobs[2][:3]) for _ in range(5)]
+        torch.cuda.synchronize()
+        for (_, out), job in zip(graphs, jobs):
+            wrong += [not torch.equal(a, b) for a, b in zip(out, job[3])]
+        for tables in got:
+            wrong += [not torch.equal(a, b) for a, b in zip(tables, jobs[2][3])]
+    assert not any(wrong)
+
+
+def test_two_calls_in_one_graph_and_the_first_call_of_a_context():
+    """A capture needs no call before it; a larger call in the same capture
+    does not take the first one's workspace away."""
+    rng = np.random.default_rng(12)
+    ctx = q3s.Context(0)
+    sizes = [(300, [90, 20], 16), (20000, [500, 300], 64), (300, [90, 20], 16)]
+    jobs = []
+    for R, vocabs, H in sizes:
+        codes = torch.from_numpy(_codes(rng, R, vocabs)).to(DEV)
+        jobs.append((codes, _grad(rng, R, H, "f32"), vocabs))
+    outs = [[torch.empty((v, j[1].shape[1]), device=DEV) for v in j[2]] for j in jobs]
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g, stream=torch.cuda.Stream()):
+        for j, out in zip(jobs, outs):
+            q3s.embed_sum_grad(*j, out=out, ctx=ctx)
+    for _ in range(3):
+        g.replay()
+    torch.cuda.synchronize()
+    for j, out in zip(jobs, outs):
+        for a, b in zip(out, q3s.embed_sum_grad(*j)):
+            assert torch.equal(a, b)
+    del g
+    torch.cuda.synchronize()
+    ctx.close()
+
+
+def test_workspaces_of_destroyed_graphs_are_used_again():
+    import gc
+    import time
+    rng = np.random.default_rng(13)
+    ctx = q3s.Context(0)
+    vocabs = [3000, 2000]
+    codes = torch.from_numpy(_codes(rng, 60000, vocabs)).to(torch.int32).to(DEV)
+    grad = _grad(rng, 60000, 512, "f32")
+    want = q3s.embed_sum_grad(codes, grad, vocabs)
+    stream, free = torch.cuda.Stream(), []
+    for _ in range(6):
+        g, out = _captured(codes, grad, vocabs, stream, ctx)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+        free.append(torch.cuda.mem_get_info(DEV)[0])
+        del g, out
+        gc.collect()
+        torch.cuda.synchronize()
+        time.sleep(0.1)  # what a graph holds may be let go on a thread of the driver's
+    # One workspace is tens of MB; six graphs one after another have one between them.
+    assert free[1] - free[-1] < 8 << 20
+    ctx.close()
