@@ -25,7 +25,10 @@ int fail(int code, const std::string& msg) {
   return code;
 }
 
+// Also takes the error back from the runtime, which would else hand it to the next
+// call that asks whether its launch succeeded.
 int cuda_fail(cudaError_t e, const char* what) {
+  cudaGetLastError();
   std::string m = std::string(what) + ": " + cudaGetErrorName(e) + " (" + cudaGetErrorString(e) + ")";
   return fail(e == cudaErrorMemoryAllocation ? Q3S_E_OUT_OF_MEMORY : Q3S_E_CUDA, m);
 }

@@ -514,3 +514,28 @@ def test_workspaces_of_destroyed_graphs_are_used_again():
     # One workspace is tens of MB; six graphs one after another have one between them.
     assert free[1] - free[-1] < 8 << 20
     ctx.close()
+
+
+def test_a_workspace_that_cannot_be_had_leaves_no_error_behind():
+    """32 codebooks of 2^31 - 1 ids need a workspace of some 550 GB: refused
+    before any launch, and the next call works."""
+    import ctypes
+    lib, ctx = q3s.load(), q3s.Context(0)
+    codes = torch.zeros((3, 32), dtype=torch.int32, device=DEV)
+    grad = torch.ones((3, 1), device=DEV)
+    # Addresses of tables that do not exist: nothing is launched.
+    ptrs = (ctypes.c_void_p * 32)(*[(1 << 44) + (k << 34) for k in range(32)])
+    sizes = (ctypes.c_int32 * 32)(*[2 ** 31 - 1] * 32)
+    b = q3s._EmbedGradBatch(dtype=0, grads_dtype=0, ids_type=1, groups=32, hidden=1, num_rows=3,
+                            codes=codes.data_ptr(), codes_stride=32, grad_out=grad.data_ptr(),
+                            grad_stride=1, grads=ctypes.addressof(ptrs),
+                            vocab=ctypes.addressof(sizes), padding_id=-1, scale=1.0)
+    torch.cuda.synchronize()
+    for _ in range(2):
+        assert lib.q3s_embed_grad(ctx.handle, ctypes.byref(b), None) == q3s.E_OUT_OF_MEMORY
+        assert "cudaMalloc" in q3s.last_error()
+        got = q3s.embed_grad(codes[:, 0].contiguous(), grad, 2, ctx=ctx)
+        assert got.tolist() == [[3.0], [0.0]]
+        out, st = q3s.embed_lookup(codes[:, 0].contiguous(), grad, ctx=ctx)
+        assert out.tolist() == [[1.0]] * 3 and st.tolist() == [0, 0, 0]
+    ctx.close()
