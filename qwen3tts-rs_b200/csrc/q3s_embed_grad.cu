@@ -74,6 +74,9 @@ struct GradArgs {
   int chunk;  // consecutive codes per warp, at most 32
 };
 
+// What a kernel writes that the next one reads is read by ordinary loads or __ldcg: the
+// next one starts before it is written, and __ldg is for memory that nothing writes
+// while the kernel lives.
 __device__ __forceinline__ void await_inputs() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void admit_next() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -140,7 +143,7 @@ __device__ __forceinline__ void load_keys(const GradArgs& a, int g, long long k,
   if (!DIRECT) {
 #pragma unroll
     for (int j = 0; j < BATCH; ++j)
-      key[j] = k + j * 32 < k1 ? __ldg(a.work[g].keys + k + j * 32) : DROPPED;
+      key[j] = k + j * 32 < k1 ? __ldcg(a.work[g].keys + k + j * 32) : DROPPED;
     return;
   }
   uint64_t c[BATCH];
@@ -463,7 +466,7 @@ struct Rows {
     base = static_cast<const char*>(b.grad_out) + (long long)col * width<T::IN>;
     stride = b.grad_stride * width<T::IN>;
     ring = (uint32_t)__cvta_generic_to_shared(ring_) + lane * T::BYTES;
-    next = k0 + lane < k1 ? __ldg(rows + k0 + lane) : 0;
+    next = k0 + lane < k1 ? __ldcg(rows + k0 + lane) : 0;
 #pragma unroll
     for (int j = 0; j < T::NV; ++j) there[j] = col + j * 32 * T::VE < b.hidden;
     if (T::ASYNC)
@@ -474,7 +477,7 @@ struct Rows {
     if (taken % 32 == 0) {
       window = next;
       const uint32_t q = issued + 32 + threadIdx.x % 32;
-      next = q < k1 ? __ldg(rows + q) : 0;
+      next = q < k1 ? __ldcg(rows + q) : 0;
     }
     const uint32_t row = __shfl_sync(0xFFFFFFFFu, window, taken % 32);
     ++issued;
