@@ -368,7 +368,9 @@ int q3s_embed_lookup(q3s_context* ctx, const q3s_lookup_batch* batch, void* stre
  * identity.  text_grad (optional) is the gradient of its text operand:
  * grad_out on valid rows and zero elsewhere for a text per row, the sum over
  * the valid rows for a broadcast one (text_stride 0); it has grads_dtype, is
- * not scaled and not accumulated.
+ * not scaled and not accumulated.  The gradients must not overlap one another
+ * (INVALID_ARGUMENT), nor grad_out or codes: for one table that several groups
+ * share, add up the groups' gradients.
  *
  * The workspace belongs to the context and grows on demand.  Direct calls on
  * one stream share one; a captured call has one of its own, so that replays may

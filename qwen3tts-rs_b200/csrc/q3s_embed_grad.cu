@@ -17,6 +17,7 @@
 // cannot be done without: each row of grad_out once and the tables once.  A row
 // is read once for each group; the groups' reads of rows that are still in L2
 // count against L2.  Each kernel starts while the one before it ends.
+#include <algorithm>
 #include <cstdint>
 #include <mutex>
 #include <string>
@@ -785,6 +786,27 @@ int bad(const char* msg) {
   return record_error(Q3S_E_INVALID_ARGUMENT, std::string("q3s_embed_grad: ") + msg);
 }
 
+// Whether two of the call's outputs share memory: two groups would write, or with
+// accumulate read and write, the same table at the same time.
+bool overlapping(const q3s_embed_grad_batch* b, int width) {
+  struct Span {
+    uintptr_t start;
+    uint64_t bytes;
+  } spans[Q3S_MAX_CODE_GROUPS + 1];
+  int n = 0;
+  for (; n < b->groups; ++n)
+    spans[n] = {reinterpret_cast<uintptr_t>(b->grads[n]), (uint64_t)b->vocab[n] * b->hidden * width};
+  if (b->text_grad && (b->text_stride == 0 || b->num_rows > 0)) {
+    const uint64_t before = b->text_stride ? (uint64_t)(b->num_rows - 1) * b->text_stride : 0;
+    spans[n++] = {reinterpret_cast<uintptr_t>(b->text_grad), (before + b->hidden) * width};
+  }
+  const auto before = [](const Span& x, const Span& y) { return x.start < y.start; };
+  if (!std::is_sorted(spans, spans + n, before)) std::sort(spans, spans + n, before);
+  for (int k = 1; k < n; ++k)
+    if (spans[k].start - spans[k - 1].start < spans[k - 1].bytes) return true;
+  return false;
+}
+
 int check(const q3s_embed_grad_batch* b) {
   if (b->num_rows < 0 || b->num_rows > 0x7FFFFFFF) return bad("num_rows must be in 0..2^31 - 1");
   if ((b->dtype != Q3S_DTYPE_F32 && b->dtype != Q3S_DTYPE_BF16) ||
@@ -813,6 +835,7 @@ int check(const q3s_embed_grad_batch* b) {
     if (off(b->grads[g], out)) return bad("a gradient table is not aligned to its elements");
     if (b->vocab[g] < 1) return bad("a codebook vocabulary is < 1");
   }
+  if (overlapping(b, out)) return bad("the gradients must not overlap one another");
   return Q3S_OK;
 }
 

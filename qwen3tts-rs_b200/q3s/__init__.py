@@ -1440,6 +1440,8 @@ def _embed_grad(dev, codes, codes_stride, grad, R, G, H, grad_stride, sizes, sca
                 raise ValueError("gradient tables must be contiguous [vocab, H] tensors of one "
                                  "type on the codes' device")
         ptrs = [t.data_ptr() for t in tables]
+        if len(set(ptrs)) != G:
+            raise ValueError("every group needs a gradient table of its own")
     text_grad, p_text, text_stride = None, 0, 0
     if text is not None:
         text_grad = _new(grad, (R, H) if text == "rows" else (H,), dt, stream)

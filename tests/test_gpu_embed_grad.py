@@ -539,3 +539,44 @@ def test_a_workspace_that_cannot_be_had_leaves_no_error_behind():
         out, st = q3s.embed_lookup(codes[:, 0].contiguous(), grad, ctx=ctx)
         assert out.tolist() == [[1.0]] * 3 and st.tolist() == [0, 0, 0]
     ctx.close()
+
+
+def test_gradients_that_overlap_are_refused():
+    """Two groups that write one table, wholly or in part, or the text's
+    gradient inside a table; tables that touch are fine, in any order."""
+    import ctypes
+    lib, ctx = q3s.load(), q3s.default_context(0)
+    R, H, sizes = 5, 8, (4, 6, 5)
+    codes = torch.randint(0, 4, (R, 3), dtype=torch.int32, device=DEV)
+    grad = torch.randn((R, H), device=DEV)
+    want = q3s.embed_sum_grad(codes, grad, sizes)
+    flat = torch.zeros((60, H), device=DEV)
+    vocab = (ctypes.c_int32 * 3)(*sizes)
+
+    def call(rows, accumulate=0, **fields):
+        flat.zero_()
+        ptrs = (ctypes.c_void_p * 3)(*[flat[r].data_ptr() for r in rows])
+        b = q3s._EmbedGradBatch(dtype=0, grads_dtype=0, ids_type=1, groups=3, hidden=H, num_rows=R,
+                                accumulate=accumulate, codes=codes.data_ptr(), codes_stride=3,
+                                grad_out=grad.data_ptr(), grad_stride=H,
+                                grads=ctypes.addressof(ptrs), vocab=ctypes.addressof(vocab),
+                                padding_id=-1, scale=1.0, **fields)
+        return lib.q3s_embed_grad(ctx.handle, ctypes.byref(b), None)
+
+    for rows in ((0, 4, 10), (11, 5, 0), (20, 0, 6)):
+        assert call(rows) == q3s.OK
+        for r, t in zip(rows, want):
+            assert torch.equal(flat[r:r + len(t)], t)
+    text = dict(text_grad=flat[40].data_ptr(), text_stride=H)
+    assert call((0, 4, 10), **text) == q3s.OK and call((35, 45, 30), **text) == q3s.OK
+    for rows in ((0, 0, 10), (0, 3, 10), (10, 4, 0), (9, 0, 5), (0, 20, 4 + 20)):
+        for accumulate in (0, 1):
+            assert call(rows, accumulate) == q3s.E_INVALID_ARGUMENT, rows
+            assert "overlap" in q3s.last_error()
+    for rows in ((0, 35, 10), (44, 4, 10)):  # rows 40..44 are the text's
+        assert call(rows, **text) == q3s.E_INVALID_ARGUMENT, rows
+    assert call((0, 38, 10), text_grad=flat[40].data_ptr(), text_stride=0) == q3s.E_INVALID_ARGUMENT
+    torch.cuda.synchronize()
+    one = torch.zeros((4, H), device=DEV)
+    with pytest.raises(ValueError, match="table of its own"):
+        q3s.embed_sum_grad(codes[:, :2], grad, [4, 4], out=[one, one], accumulate=True)
