@@ -337,7 +337,7 @@ typedef struct q3s_lookup_batch {
   int32_t dtype;     /* Q3S_DTYPE_* of table */
   int32_t out_dtype; /* Q3S_DTYPE_* of out */
   int32_t ids_type;  /* Q3S_IDS_* */
-  int32_t hidden;    /* elements per row, >= 1 */
+  int32_t hidden;    /* elements per row, 1..2^30 */
   int64_t vocab;     /* rows of table, >= 1 */
   int64_t num_ids;
   const void* ids;       /* [num_ids] */

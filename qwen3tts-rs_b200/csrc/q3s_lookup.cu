@@ -19,6 +19,7 @@ namespace q3s {
 namespace {
 
 constexpr int THREADS = 256;
+constexpr int MAX_HIDDEN = 1 << 30;  // 32-bit counters of a row's vectors go somewhat beyond its end
 
 template <int DT>
 constexpr int width = DT == Q3S_DTYPE_F32 ? 4 : 2;  // bytes of an element
@@ -101,7 +102,7 @@ __global__ void __launch_bounds__(THREADS) lookup_kernel(const LookupArgs a) {
 #pragma unroll
       for (int j = 0; j < AHEAD; ++j) {
         const int v = v0 + j * a.lanes;
-        if (v < a.vectors && !zero) x[j].load(src + v * VE * width<IN>);
+        if (v < a.vectors && !zero) x[j].load(src + (long long)v * (VE * width<IN>));
       }
 #pragma unroll
       for (int j = 0; j < AHEAD; ++j) {
@@ -110,7 +111,7 @@ __global__ void __launch_bounds__(THREADS) lookup_kernel(const LookupArgs a) {
         Raw<OUT, VE> y;
 #pragma unroll
         for (int e = 0; e < VE; ++e) y.set(e, zero ? 0.0f : __fmul_rn(x[j].at(e), b.scale));
-        y.store(dst + v * VE * width<OUT>);
+        y.store(dst + (long long)v * (VE * width<OUT>));
       }
     }
   }
@@ -154,7 +155,8 @@ int embed_lookup(q3s_context* ctx, const q3s_lookup_batch* b, void* stream) {
     return bad("dtype and out_dtype must be Q3S_DTYPE_F32 or Q3S_DTYPE_BF16");
   if (b->ids_type != Q3S_IDS_U16 && b->ids_type != Q3S_IDS_U32 && b->ids_type != Q3S_IDS_I64)
     return bad("unknown ids_type");
-  if (b->hidden < 1 || b->vocab < 1) return bad("hidden and vocab must be >= 1");
+  if (b->hidden < 1 || b->hidden > MAX_HIDDEN) return bad("hidden must be in 1..2^30");
+  if (b->vocab < 1) return bad("vocab must be >= 1");
   if (b->table_stride < b->hidden || b->out_stride < b->hidden)
     return bad("table_stride and out_stride must be >= hidden");
   if (b->num_ids == 0) return Q3S_OK;

@@ -199,3 +199,36 @@ def test_the_c_entry_refuses():
         assert "q3s_embed_lookup" in q3s.last_error()
     assert lib.q3s_embed_lookup(None, None, None) == q3s.E_INVALID_ARGUMENT
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("H", [2 ** 29 + 8, 2 ** 29 + 9])
+def test_rows_longer_than_2_gib(H):
+    """Offsets inside one row pass 31 bits: f32 rows of 2 GiB and a little,
+    in vectors and in single elements."""
+    table = torch.empty((2, H), device=DEV)
+    table[:, :1024], table[:, 1024:-1024], table[:, -1024:] = 1.0, 2.0, 3.0
+    table[1, -1] = 5.0
+    out, st = q3s.embed_lookup(torch.tensor([1, 0], device=DEV), table, 0.5)
+    assert st.tolist() == [0, 0]
+    for k in (0, 1):
+        for part in (slice(0, 1024), slice(1024, H - 1024), slice(H - 1024, H)):
+            a, b = out[k, part], table[1 - k, part]
+            for lo in range(0, len(a), 1 << 27):
+                assert torch.equal(a[lo:lo + (1 << 27)], b[lo:lo + (1 << 27)] * 0.5)
+    del table, out
+    torch.cuda.empty_cache()
+
+
+def test_the_longest_rows():
+    ids = torch.zeros(1, dtype=torch.int64, device=DEV)
+    x = torch.zeros((1, 8), device=DEV)
+    st = torch.zeros(1, dtype=torch.uint8, device=DEV)
+    b = q3s._LookupBatch(dtype=0, out_dtype=0, ids_type=2, hidden=2 ** 30 + 1, vocab=1, num_ids=0,
+                         ids=ids.data_ptr(), table=x.data_ptr(), table_stride=2 ** 31,
+                         out=x.data_ptr(), out_stride=2 ** 31, scale=1.0, status=st.data_ptr())
+    import ctypes
+    call = lambda: q3s.load().q3s_embed_lookup(q3s.default_context(0).handle,  # noqa: E731
+                                               ctypes.byref(b), None)
+    assert call() == q3s.E_INVALID_ARGUMENT and "hidden" in q3s.last_error()
+    b.hidden = 2 ** 30
+    assert call() == q3s.OK  # no ids: nothing is launched
