@@ -383,7 +383,7 @@ typedef struct q3s_embed_grad_batch {
   int32_t grads_dtype; /* Q3S_DTYPE_* of grads and text_grad */
   int32_t ids_type;    /* Q3S_IDS_* of codes */
   int32_t groups;      /* G, 1..Q3S_MAX_CODE_GROUPS */
-  int32_t hidden;      /* H, >= 1 */
+  int32_t hidden;      /* H, 1..2^30 */
   int32_t accumulate;  /* 0: grads are overwritten, else added to */
   int64_t num_rows;    /* R, 0..2^31 - 1 */
   const void* codes;     /* [R, codes_stride], G ids a row */

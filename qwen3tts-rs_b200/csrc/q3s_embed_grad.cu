@@ -48,6 +48,7 @@ constexpr int TEXT_THREADS = 256;
 constexpr int REDUCE_THREADS = 128;
 constexpr int REDUCE_WARPS = REDUCE_THREADS / 32;
 constexpr uint32_t DROPPED = 0xFFFFFFFFu;
+constexpr int MAX_HIDDEN = 1 << 30;  // 32-bit columns of a row's tiles go somewhat beyond its end
 constexpr int JOIN = 16;           // pieces of a long run that one warp joins
 constexpr uint32_t GROUPS = 1u << 16;  // `arrived` counts pieces below it, groups of them from it on
 
@@ -174,7 +175,7 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(const GradArgs a) {
   const int block = MANY ? (int)cluster.block_rank() : 0;
   const int g = blockIdx.y, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int bucket = 1 << a.bucket_bits, vocab = a.vocab[g];
-  const int buckets = (vocab + bucket - 1) >> a.bucket_bits;
+  const int buckets = (int)(((long long)vocab + bucket - 1) >> a.bucket_bits);
   admit_next();
   if ((int)blockIdx.x / blocks >= buckets) return;  // the whole cluster
   const GroupWork& w = a.work[g];
@@ -187,8 +188,8 @@ __global__ void __launch_bounds__(SORT_THREADS) sort_kernel(const GradArgs a) {
   uint32_t* mine = hist + (warp << a.bucket_bits);
   for (int i = threadIdx.x; i < SORT_WARPS << a.bucket_bits; i += SORT_THREADS) hist[i] = 0;
   if (!DIRECT) await_inputs();
-  for (int i = blockIdx.x * SORT_THREADS + threadIdx.x; i < a.slots;
-       i += buckets * blocks * SORT_THREADS)
+  for (long long i = blockIdx.x * (long long)SORT_THREADS + threadIdx.x; i < a.slots;
+       i += (long long)buckets * blocks * SORT_THREADS)
     w.arrived[i] = 0;
   __syncthreads();
   // Every warp counts consecutive rows: its bucket's codes, and all below.
@@ -815,7 +816,7 @@ int check(const q3s_embed_grad_batch* b) {
   if (b->ids_type != Q3S_IDS_U16 && b->ids_type != Q3S_IDS_U32 && b->ids_type != Q3S_IDS_I64)
     return bad("unknown ids_type");
   if (b->groups < 1 || b->groups > Q3S_MAX_CODE_GROUPS) return bad("groups must be in 1..32");
-  if (b->hidden < 1) return bad("hidden must be >= 1");
+  if (b->hidden < 1 || b->hidden > MAX_HIDDEN) return bad("hidden must be in 1..2^30");
   if (!b->grads || !b->vocab) return bad("grads and vocab are required");
   if (b->num_rows > 0) {
     if (!b->codes || !b->grad_out) return bad("codes and grad_out are required");
@@ -850,7 +851,7 @@ cudaError_t launch_sums(const GradArgs& a, int groups, int max_vocab, int device
   static std::atomic<uint64_t> allowed{0};
   const cudaError_t e = allow_smem((const void*)reduce_kernel<T, OUT>, T::SMEM, device, allowed);
   if (e != cudaSuccess) return e;
-  const long long warps = (a.blocks + (max_vocab + a.chunk - 1LL) / a.chunk) * a.tiles;
+  const long long warps = (a.blocks + ((long long)max_vocab + a.chunk - 1) / a.chunk) * a.tiles;
   const dim3 grid((unsigned)((warps + REDUCE_WARPS - 1) / REDUCE_WARPS), groups);
   const cudaError_t l = launch_after(reduce_kernel<T, OUT>, grid, REDUCE_THREADS, T::SMEM, st, true, 0, a);
   if (l != cudaSuccess) return l;

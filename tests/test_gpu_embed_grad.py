@@ -580,3 +580,31 @@ def test_gradients_that_overlap_are_refused():
     one = torch.zeros((4, H), device=DEV)
     with pytest.raises(ValueError, match="table of its own"):
         q3s.embed_sum_grad(codes[:, :2], grad, [4, 4], out=[one, one], accumulate=True)
+
+
+def test_the_largest_table():
+    """2^31 - 1 ids: the counts of buckets and blocks pass 31 bits."""
+    V = 2 ** 31 - 1
+    ids = torch.tensor([0, V - 1, 5, V - 1, 2 ** 30, V - 1025, V - 1024, 5], device=DEV)
+    grad = torch.arange(1, 9, device=DEV, dtype=torch.float32)[:, None].bfloat16()
+    ctx = q3s.Context(0)  # its workspace holds a range for each id: 17 GB
+    got = q3s.embed_grad(ids.to(torch.int32), grad, V, ctx=ctx)[:, 0]
+    want = {0: 1, V - 1: 6, 5: 11, 2 ** 30: 5, V - 1025: 6, V - 1024: 7}
+    assert {k: float(got[k]) for k in want} == want
+    assert sum(int(torch.count_nonzero(p)) for p in got.split(1 << 28)) == len(want)
+    ctx.close()
+    del got
+    torch.cuda.empty_cache()
+
+
+def test_the_longest_rows():
+    """hidden beyond 2^30 is refused (num_rows 0: nothing would be read)."""
+    import ctypes
+    out = torch.zeros((1, 8), device=DEV)
+    ptrs, sizes = (ctypes.c_void_p * 1)(out.data_ptr()), (ctypes.c_int32 * 1)(1)
+    b = q3s._EmbedGradBatch(dtype=0, grads_dtype=0, ids_type=1, groups=1, hidden=2 ** 30 + 1,
+                            num_rows=0, accumulate=1, grads=ctypes.addressof(ptrs),
+                            vocab=ctypes.addressof(sizes), padding_id=-1, scale=1.0)
+    lib, ctx = q3s.load(), q3s.default_context(0)
+    assert lib.q3s_embed_grad(ctx.handle, ctypes.byref(b), None) == q3s.E_INVALID_ARGUMENT
+    assert "hidden" in q3s.last_error()
