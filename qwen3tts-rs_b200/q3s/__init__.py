@@ -1524,21 +1524,42 @@ def _functions() -> dict:
         return _autograd
     import torch
 
+    def rows(t):
+        """t, with contiguous rows that do not overlap."""
+        good = t.dim() <= 2 and t.stride(-1) == 1 and (t.dim() == 1 or t.stride(0) >= t.shape[1])
+        return t if good else t.contiguous()
+
+    def lookup_grad(ids, grad, vocab, scale, padding_id):
+        if grad.stride(-1) != 1 or grad.dim() > 2:
+            grad = grad.contiguous()
+        return embed_grad(ids, grad, vocab, scale, padding_id)
+
+    # Each gradient is linear in what it is taken of, and the other function's
+    # forward pass is its own gradient: both differentiate any number of times.
     class Embedding(torch.autograd.Function):
         @staticmethod
         def forward(c, ids, table, scale, padding_id):
             c.save_for_backward(ids)
-            c.args = (table.shape[0], scale, padding_id, table.dtype)
+            c.args = (table.shape[0], scale, padding_id)
             return embed_lookup(ids, table, scale, padding_id)[0]
 
         @staticmethod
         def backward(c, grad):
             (ids,) = c.saved_tensors
-            vocab, scale, padding_id, dtype = c.args
-            if grad.stride(-1) != 1 or grad.dim() > 2:
-                grad = grad.contiguous()
-            return None, embed_grad(ids, grad, vocab, scale, padding_id, out_dtype=dtype), None, \
-                None
+            got = EmbeddingGrad.apply if torch.is_grad_enabled() else lookup_grad  # create_graph
+            return None, got(ids, grad, *c.args), None, None
+
+    class EmbeddingGrad(torch.autograd.Function):
+        @staticmethod
+        def forward(c, ids, grad, vocab, scale, padding_id):
+            c.save_for_backward(ids)
+            c.args = (scale, padding_id)
+            return lookup_grad(ids, grad, vocab, scale, padding_id)
+
+        @staticmethod
+        def backward(c, grad):
+            (ids,) = c.saved_tensors
+            return None, Embedding.apply(ids, rows(grad), *c.args), None, None, None
 
     class CodebookEmbedding(torch.autograd.Function):
         @staticmethod
@@ -1553,11 +1574,34 @@ def _functions() -> dict:
         def backward(c, grad):
             (codes,) = c.saved_tensors
             want = c.text if c.needs_input_grad[1] else None
+            if torch.is_grad_enabled():  # create_graph
+                got = CodebookGrad.apply(codes, grad, c.vocabs, want)
+                return (None, None if want is None else got[-1], *got[:len(c.vocabs)])
             if grad.stride(1) != 1:
                 grad = grad.contiguous()
             got = embed_sum_grad(codes, grad, c.vocabs, text=want)
             tables, text = (got, None) if want is None else got
             return (None, text, *tables)
+
+    class CodebookGrad(torch.autograd.Function):
+        """The tables' gradients, and the text's behind them."""
+
+        @staticmethod
+        def forward(c, codes, grad, vocabs, want):
+            c.save_for_backward(codes)
+            c.groups = len(vocabs)
+            grad = rows(grad)
+            # Tables of their own: one output must not be a view of another's memory.
+            out = [grad.new_empty((v, grad.shape[1])) for v in vocabs]
+            got = embed_sum_grad(codes, grad, vocabs, out=out, text=want)
+            return tuple(out) if want is None else (*out, got[1])
+
+        @staticmethod
+        def backward(c, *grads):
+            (codes,) = c.saved_tensors
+            tables = [t.contiguous() for t in grads[:c.groups]]
+            text = rows(grads[c.groups]) if len(grads) > c.groups else None
+            return None, CodebookEmbedding.apply(codes, text, *tables), None, None
 
     _autograd.update(embedding=Embedding, codebook=CodebookEmbedding)
     return _autograd
@@ -1566,11 +1610,12 @@ def _functions() -> dict:
 def embedding(ids, table, scale: float = 1.0, padding_id: Optional[int] = None):
     """embed_lookup for torch's autograd: the looked-up rows, whose gradient
     reaches `table` through embed_grad.  An id outside the table gives zeros
-    and no gradient."""
+    and no gradient.  Derivatives of any order (create_graph)."""
     return _functions()["embedding"].apply(ids, table, float(scale), padding_id)
 
 
 def codebook_embedding(codes, tables, text=None):
     """embed_sum for torch's autograd: the rows, whose gradient reaches the
-    tables and the text through embed_sum_grad."""
+    tables and the text through embed_sum_grad.  Derivatives of any order
+    (create_graph)."""
     return _functions()["codebook"].apply(codes, text, *tables)

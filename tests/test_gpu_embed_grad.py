@@ -608,3 +608,69 @@ def test_the_longest_rows():
     lib, ctx = q3s.load(), q3s.default_context(0)
     assert lib.q3s_embed_grad(ctx.handle, ctypes.byref(b), None) == q3s.E_INVALID_ARGUMENT
     assert "hidden" in q3s.last_error()
+
+
+def _loss_with_its_own_gradient(rows, tensors):
+    """sum rows^3, plus the squares of its own gradient, plus the cubes of that
+    gradient's: derivatives up to the third.  Small whole numbers, so every
+    product and sum is exact in f32."""
+    loss = (rows ** 3).sum()
+    first = torch.autograd.grad(loss, tensors, create_graph=True)
+    assert all(g.requires_grad for g in first)
+    second = torch.autograd.grad(sum((g ** 2).sum() for g in first), tensors, create_graph=True)
+    return loss + sum((g * w).sum() for g, w in zip(second, tensors))
+
+
+def test_second_and_third_derivatives_of_the_lookup():
+    """Against torch's own embedding in 64 bits; a padding id and an id that
+    the table does not have."""
+    rng = np.random.default_rng(14)
+    V, H, pad = 6, 5, 2
+    ids = torch.tensor([[0, 1, 1], [2, 5, 6]], device=DEV)
+    table = torch.from_numpy(rng.integers(-1, 2, (V, H))).float().to(DEV).requires_grad_()
+    x = q3s.embedding(ids, table, 2.0, padding_id=pad)
+    _loss_with_its_own_gradient(x, [table]).backward()
+    want = table.detach().double().requires_grad_()
+    live = ((ids != pad) & (ids < V)).double()[..., None]
+    y = torch.nn.functional.embedding(ids.clamp(max=V - 1), want) * 2.0 * live
+    _loss_with_its_own_gradient(y, [want]).backward()
+    assert torch.equal(table.grad.double(), want.grad)
+    assert float(want.grad.abs().max()) < 2 ** 24
+
+
+@pytest.mark.parametrize("shape", [None, (12, 4), (4,)])
+def test_second_and_third_derivatives_of_the_codebook_sum(shape):
+    """With no text, one per row and one for all; a row with a code that its
+    codebook does not have."""
+    rng = np.random.default_rng(15)
+    vocabs, R, H = [3, 5], 12, 4
+    codes = _codes(rng, R, vocabs)
+    codes[7, 1] = 5
+    dev = torch.from_numpy(codes).to(torch.int32).to(DEV)
+    tensors = [torch.from_numpy(rng.integers(-1, 2, (v, H))).float().to(DEV).requires_grad_()
+               for v in vocabs]
+    if shape is not None:
+        tensors.append(torch.from_numpy(rng.integers(-1, 2, shape)).float().to(DEV).requires_grad_())
+    x = q3s.codebook_embedding(dev, tensors[:2], tensors[2] if shape else None)
+    _loss_with_its_own_gradient(x, tensors).backward()
+    want = [t.detach().double().requires_grad_() for t in tensors]
+    live = torch.ones((R, 1), dtype=torch.float64, device=DEV)
+    live[7] = 0
+    y = sum(want[g][torch.from_numpy(codes[:, g].clip(0, v - 1)).to(DEV)] for g, v in enumerate(vocabs))
+    y = (y + want[2] if shape else y) * live
+    _loss_with_its_own_gradient(y, want).backward()
+    for a, b in zip(tensors, want):
+        assert float(b.grad.abs().max()) < 2 ** 24
+        assert torch.equal(a.grad.double(), b.grad)
+
+
+def test_a_penalty_on_the_gradient_reaches_only_what_trains():
+    """One frozen table and a text that does not train, with create_graph."""
+    codes = torch.tensor([[0, 1], [1, 1]], dtype=torch.int32, device=DEV)
+    a = torch.ones((2, 3), device=DEV, requires_grad=True)
+    b, text = torch.ones((2, 3), device=DEV), torch.ones(3, device=DEV)
+    x = q3s.codebook_embedding(codes, [a, b], text)
+    (g,) = torch.autograd.grad((x ** 2).sum(), [a], create_graph=True)
+    (g ** 2).sum().backward()
+    # g = 2 (a + b + text) a row, its square's derivative 2 g 2
+    assert torch.equal(a.grad, torch.full((2, 3), 24.0, device=DEV)) and b.grad is None
