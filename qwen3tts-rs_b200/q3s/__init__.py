@@ -1409,8 +1409,8 @@ def _embed_grad(dev, codes, codes_stride, grad, R, G, H, grad_stride, sizes, sca
         raise ValueError("grad must have contiguous rows that do not overlap")
     if not 1 <= G <= MAX_CODE_GROUPS or len(sizes) != G:
         raise ValueError("one vocabulary per code group (1..32)")
-    if min(sizes) < 1:
-        raise ValueError("every vocabulary must be >= 1")
+    if min(sizes) < 1 or max(sizes) >= 2 ** 31:  # a C int holds it, and would wrap silently
+        raise ValueError("every vocabulary must be in 1..2^31 - 1")
     dtype = _float_type(grad.dtype, "grad")
     ids_type = _ids_type(codes.dtype, "codes")
     if out is None:

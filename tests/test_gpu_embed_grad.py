@@ -674,3 +674,15 @@ def test_a_penalty_on_the_gradient_reaches_only_what_trains():
     (g ** 2).sum().backward()
     # g = 2 (a + b + text) a row, its square's derivative 2 g 2
     assert torch.equal(a.grad, torch.full((2, 3), 24.0, device=DEV)) and b.grad is None
+
+
+def test_vocabularies_beyond_31_bits_are_refused():
+    """2^32 + 5 must not pass for 5."""
+    ids = torch.zeros(3, dtype=torch.int64, device=DEV)
+    grad = torch.zeros((3, 1), device=DEV)
+    codes = torch.zeros((3, 2), dtype=torch.int32, device=DEV)
+    for vocab in (2 ** 31, 2 ** 32 + 5):
+        with pytest.raises(ValueError, match="vocabulary"):
+            q3s.embed_grad(ids, grad, vocab)
+        with pytest.raises(ValueError, match="vocabulary"):
+            q3s.embed_sum_grad(codes, grad, [4, vocab])
