@@ -686,3 +686,57 @@ def test_vocabularies_beyond_31_bits_are_refused():
             q3s.embed_grad(ids, grad, vocab)
         with pytest.raises(ValueError, match="vocabulary"):
             q3s.embed_sum_grad(codes, grad, [4, vocab])
+
+
+def _check_large(tables, codes, grad, vocabs):
+    """_check for many rows: the same sums and the same bound, on the device."""
+    dev = torch.from_numpy(codes).to(DEV)
+    g64 = grad.double()
+    for g, v in enumerate(vocabs):
+        value, size = (torch.zeros((v, grad.shape[1]), dtype=torch.float64, device=DEV).index_add_(
+            0, dev[:, g], x) for x in (g64, g64.abs()))
+        count = torch.bincount(dev[:, g], minlength=v).double()
+        bound = 1.01 * (2 * so.U * (count - 1).clamp(min=0)[:, None] * size + so.U * value.abs())
+        bf16 = tables[g].dtype == torch.bfloat16
+        so.check(tables[g].double().cpu().numpy(), value.cpu().numpy(),
+                 so.rounded(bound.cpu().numpy(), value.cpu().numpy(), bf16), f"group {g}")
+        assert (tables[g][count == 0] == 0).all()
+
+
+@pytest.mark.parametrize("R,vocabs,hot", [
+    (70000, [100003], 0.5),       # one block a bucket; warps that find more keys than they keep
+    (70000, [100003], 0.0),
+    (140000, [500], 0.97),        # clusters of eight, the same
+    (140000, [500, 40], 0.97),    # several groups
+    (140000, [500, 40], 0.0),
+    (33000, [2000], 0.3),         # clusters of eight, lists that suffice
+    (2000, [152000], 0.1),        # more buckets than multiprocessors
+])
+def test_sorts_of_many_rows(R, vocabs, hot):
+    """Each way the sort goes with many rows, and pieces of more than 32
+    rows (above 65536)."""
+    rng = np.random.default_rng(R + len(vocabs))
+    codes = _codes(rng, R, vocabs, 2.0)
+    codes[rng.random(R) < hot] = np.array(vocabs) - 1
+    grad = _grad(rng, R, 4, "f32")
+    dev = torch.from_numpy(codes).to(torch.int32).to(DEV)
+    got = [q3s.embed_grad(dev[:, 0].contiguous(), grad, vocabs[0])] if len(vocabs) == 1 else \
+        q3s.embed_sum_grad(dev, grad, vocabs)
+    _check_large(got, codes, grad, vocabs)
+
+
+@pytest.mark.parametrize("out", ["f32", "bf16"])
+@pytest.mark.parametrize("H", [256, 512, 1024, 1280])
+def test_long_runs_of_wide_bf16_rows(H, out):
+    """A code with most of 6001 rows: pieces joined in two steps, in tiles of
+    one, two and four 16-byte vectors a lane."""
+    rng = np.random.default_rng(H)
+    R, vocabs = 6001, [300, 50]
+    codes = _codes(rng, R, vocabs)
+    codes[rng.random(R) < 0.8] = [299, 17]
+    grad = _grad(rng, R, H, "bf16")
+    dev = torch.from_numpy(codes).to(torch.int32).to(DEV)
+    got = q3s.embed_sum_grad(dev, grad, vocabs, out_dtype=TYPES[out])
+    _check_large(got, codes, grad, vocabs)
+    one = q3s.embed_grad(dev[:, 0].contiguous(), grad, 300, out_dtype=TYPES[out])
+    assert torch.equal(one, got[0])
