@@ -385,7 +385,7 @@ typedef struct q3s_embed_grad_batch {
   int32_t groups;      /* G, 1..Q3S_MAX_CODE_GROUPS */
   int32_t hidden;      /* H, 1..2^30 */
   int32_t accumulate;  /* 0: grads are overwritten, else added to */
-  int64_t num_rows;    /* R, 0..2^31 - 1 */
+  int64_t num_rows;    /* R, 0..2^31 - 1; R times the sum of vocab at most 2^48 */
   const void* codes;     /* [R, codes_stride], G ids a row */
   int64_t codes_stride;  /* elements, >= G */
   const void* grad_out;  /* [R, grad_stride] */

@@ -836,6 +836,12 @@ int check(const q3s_embed_grad_batch* b) {
     if (off(b->grads[g], out)) return bad("a gradient table is not aligned to its elements");
     if (b->vocab[g] < 1) return bad("a codebook vocabulary is < 1");
   }
+  // The sort looks at every key once for each 1024 ids: 0.43 s at this bound (2^24 rows,
+  // as many ids), and in proportion beyond it, without end for what the types hold.
+  uint64_t ids = 0;
+  for (int g = 0; g < b->groups; ++g) ids += (uint64_t)b->vocab[g];
+  if (b->num_rows && ids > (1ull << 48) / (uint64_t)b->num_rows)
+    return bad("num_rows times the sum of vocab must be at most 2^48");
   if (overlapping(b, out)) return bad("the gradients must not overlap one another");
   return Q3S_OK;
 }

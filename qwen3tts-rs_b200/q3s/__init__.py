@@ -1465,7 +1465,8 @@ def embed_grad(ids, grad, vocab: int, scale: float = 1.0, padding_id: Optional[i
     """The gradient of embed_lookup with respect to its table
     (q3s_embed_grad): row v is scale * the sum of grad over the ids equal to
     v, in f32, in an order that depends on the ids alone.  ids: any shape,
-    contiguous; grad: [..., H] of the ids' shape, float32 or bfloat16.
+    contiguous; grad: [..., H] of the ids' shape, float32 or bfloat16; ids
+    times vocab at most 2^48.
     Returns [vocab, H] in out_dtype (grad's by default), or out, overwritten
     or with accumulate added to."""
     dev = _cuda(ids, "ids")

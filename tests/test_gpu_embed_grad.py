@@ -740,3 +740,26 @@ def test_long_runs_of_wide_bf16_rows(H, out):
     _check_large(got, codes, grad, vocabs)
     one = q3s.embed_grad(dev[:, 0].contiguous(), grad, 300, out_dtype=TYPES[out])
     assert torch.equal(one, got[0])
+
+
+def test_calls_that_would_take_minutes_are_refused():
+    """The sort's time goes by rows times ids: beyond 2^48 the call is refused
+    on the host.  (32 tables of 2^31 - 1 ids: their workspace could not be had
+    either, so nothing is launched in any case.)"""
+    import ctypes
+    lib, ctx = q3s.load(), q3s.Context(0)
+    codes = torch.zeros((3, 32), dtype=torch.int32, device=DEV)
+    grad = torch.ones((3, 1), device=DEV)
+    ptrs = (ctypes.c_void_p * 32)(*[(1 << 44) + (k << 34) for k in range(32)])
+    sizes = (ctypes.c_int32 * 32)(*[2 ** 31 - 1] * 32)
+    b = q3s._EmbedGradBatch(dtype=0, grads_dtype=0, ids_type=1, groups=32, hidden=1,
+                            num_rows=2 ** 31 - 1, codes=codes.data_ptr(), codes_stride=32,
+                            grad_out=grad.data_ptr(), grad_stride=1,
+                            grads=ctypes.addressof(ptrs), vocab=ctypes.addressof(sizes),
+                            padding_id=-1, scale=1.0)
+    for rows, want in ((2 ** 31 - 1, q3s.E_INVALID_ARGUMENT), (4097, q3s.E_INVALID_ARGUMENT),
+                       (4096, q3s.E_OUT_OF_MEMORY)):
+        b.num_rows = rows
+        assert lib.q3s_embed_grad(ctx.handle, ctypes.byref(b), None) == want, rows
+        assert ("2^48" in q3s.last_error()) == (want == q3s.E_INVALID_ARGUMENT)
+    ctx.close()
