@@ -68,8 +68,8 @@ extern "C" {
 #define Q3S_DTYPE_BF16 1 /* upcast exactly to f32 before any arithmetic */
 
 /* ---- element types of ids (logits processing, embedding lookup and gradient) */
-#define Q3S_IDS_U16 0
-#define Q3S_IDS_U32 1 /* an i32 id below zero is an id that no table or vocabulary has */
+#define Q3S_IDS_U16 0 /* an i16 id below zero is one from 2^15 on */
+#define Q3S_IDS_U32 1 /* an i32 id below zero is one from 2^31 on: none of a smaller table's */
 #define Q3S_IDS_I64 2
 
 /* "None" for suppress_from / allow_suppressed_token. */

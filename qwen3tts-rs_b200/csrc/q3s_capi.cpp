@@ -142,7 +142,7 @@ namespace {
 using Used = std::shared_ptr<std::atomic<bool>>;
 
 // The destructor of the object that a captured graph holds.  It may run on a
-// thread of the driver's and after the context is gone, and calls nothing.
+// thread of CUDA's and after the context is gone, and calls nothing.
 void CUDART_CB graph_is_gone(void* p) {
   Used* used = static_cast<Used*>(p);
   (*used)->store(false);

@@ -159,9 +159,10 @@ __device__ __forceinline__ void load_keys(const GradArgs& a, int g, long long k,
   for (int j = 0; j < BATCH; ++j) key[j] = c[j] < (uint64_t)a.vocab[g] ? kept(a, c[j]) : DROPPED;
 }
 
-// Bound by the issue of the warps that look at every key of the group: 12.5 us for
-// 16384 keys and 98 buckets, 9 us for 16 groups of 4096, 18 us for 16 groups of 32768 in
-// clusters of four.  A radix sort of clusters that exchange
+// Bound by the issue of the warps that look at every key of the group: 12.7 us for
+// 16384 keys and 98 buckets, 8.6 us for 16 groups of 4096, 18 us for 16 groups of 32768 in
+// clusters of four.  One block takes a multiprocessor, so beyond 148 buckets of 1024
+// codes there is a second wave over all keys.  A radix sort of clusters that exchange
 // their digits' totals lost 24 us of 26 to the exchange and to a second wave; this one
 // tells only 1024 counts once.  Lanes with one code find each other by a ballot
 // for each bit: the instruction that matches lanes by value answers 0.9 lanes a
@@ -586,9 +587,9 @@ __device__ __forceinline__ void finish(const GradArgs& a, int g, long long v, in
 // block: slot 0 belongs to the run that holds the block's first position, slot
 // 1 to a run that starts inside the block and leaves it.  The warp that
 // finishes the last of JOIN pieces adds them up in order, and the one that finishes
-// the last of these groups the groups' sums.  (One after another, the 256 pieces of
-// a code that 32768 rows have cost 110 us, in groups of 16 40 us; groups of 8 or 32 differ
-// by less than 3 us from those of 16.)
+// the last of these groups the groups' sums.  (Groups of 8 or 32 instead of 16 change no
+// case by more than 0.5 us.  When pieces were 128 rows, 256 of them one after another
+// took 110 us, in groups of 16 40 us.)
 template <class T, int OUT>
 __device__ __forceinline__ void add_pieces(const GradArgs& a, int g, long long block, int tile,
                                            char* ring) {
@@ -661,16 +662,21 @@ __device__ __forceinline__ void add_pieces(const GradArgs& a, int g, long long b
   }
 }
 
-// Bound by HBM for a large table (16384 rows of 1024 bf16 into 100003 rows of f32, most
-// of them zeros: 72-77 us, 5.7-6.2 TB/s), by issue where rows come from L2 and codes
-// have two each (16 groups of 4096 rows of 2048 bf16: 41-46 us, 57 % of the slots), and by
-// L2 itself for more (16 groups of 32768 rows of 1024 bf16: about 130 us for 1.07 GB of
-// gathered rows, 8 TB/s).  What was measured on the way, at the last two: rings of 8
-// rows for 16: 91 to 70 and 237 to 204 us (more blocks a multiprocessor); 32 columns a
-// lane for 16: 64 to 60 and 211 to 201 us; a bf16 added to an f32 in one instruction
-// for unpacked pairs: 71 to 64 and 228 to 211 us; five blocks a multiprocessor: 57 and
-// 174 us (four 58 / 190, six 56 / 185).  Sums by matrix instructions with a selection matrix are not open: 0
-// times an infinity of another row would be NaN.
+// Counters of single cold launches.  A large table is bound by HBM (16384 rows of 1024
+// bf16 into 100003 rows of f32, most of them zeros: 77 us, 5.0 TB/s with the launch and
+// the tail in it).  Codes with two rows each, in L2, are bound by issue (16 groups of
+// 4096 rows of 2048 bf16: 47 us, 57 % of the slots, 220 instructions of a warp for a
+// row's 1024 columns).  With more rows than L2 keeps nothing is full (16 groups of 32768
+// rows of 1024 bf16, 1.07 GB gathered: 136 us, HBM at 3.0 TB/s, 52 % hits in L2 and 37 %
+// of its throughput, issue 44 %, 15 of 20 warps at work): the gathers' latency and the
+// tail are what is left.
+//
+// Whole calls, that last case and the one before: rings of 8 rows of 64 bytes a lane
+// 187 and 61 us instead of 151 and 50 with 4; four blocks a multiprocessor 172 and 52,
+// six 151 and 49; 16 columns a lane 175 and 56.  A bf16 added to an f32 in one
+// instruction took 228 to 211 and 71 to 64 us at that step.  Sums by matrix
+// instructions with a selection matrix are not open: 0 times an infinity of another row
+// would be NaN.
 //
 // A warp takes the pieces in one block of the sorted list, or the runs of a
 // chunk of consecutive codes, for one tile of columns.  The codes' runs lie one
@@ -724,7 +730,7 @@ __global__ void __launch_bounds__(REDUCE_THREADS, 5) reduce_kernel(const GradArg
 // The gradient of a text operand per row: grad_out, or zeros where the row is
 // not valid.  A warp a row: a lane looks at each of its codes, and four vectors a
 // lane are in flight.  Bound by HBM: 4096 rows of 2048 bf16 5.4 us (5.1 us at the copy
-// rate; 13.5 us with a block a row and single columns), 32768 of 1024 to f32 41 us (31).
+// rate; 13.5 us with a block a row and single columns), 32768 of 1024 to f32 40 us (31).
 template <int IN, int OUT, int VE>
 __global__ void __launch_bounds__(TEXT_THREADS) text_kernel(const GradArgs a) {
   constexpr int AHEAD = 4, SE = OUT == Q3S_DTYPE_F32 && VE == 8 ? 4 : VE;
@@ -920,15 +926,17 @@ int embed_grad(q3s_context* ctx, const q3s_embed_grad_batch* b, void* stream) {
   // Pieces of about sqrt(rows) / 8 positions, 32 at least: a warp then adds at
   // most two pieces' rows in turn, or JOIN pieces, or the groups of the longest
   // possible run (32 positions, 64, 128: 16 groups of 32768 rows, a few codes frequent,
-  // 150, 158 and 165 us, 172 us with 16; 20000 rows of 1024 f32, one group, 29, 39 and 58
-  // us; every code as frequent, 16 groups of 32768 rows, 115, 112 and 109 us).
+  // 151, 158 and 164 us; 20000 rows of 1024 f32, one group, 29, 39 and 58 us; every code
+  // as frequent, 16 groups of 32768 rows, 120, 116 and 113 us; 16 of 4096, 50, 49, 48).
+  // Their sums are most of the workspace: 4 bytes a column, two for every piece that
+  // rows can have, 134 MB for the 16 groups of 32768 rows of 1024.
   a.block = 32;
   while (64LL * a.block * a.block < b->num_rows) a.block *= 2;
   const int ve = vector_columns(a, groups);
   // As many 16-byte vectors a lane, up to four, as leave no lane idle (what a row
   // costs besides its columns is then shared by more of them: at most two instead of
-  // four, 48 -> 56 us for 16 groups of 4096 rows of 2048 bf16, 162 -> 171 us for 32768 of
-  // 1024, no difference for text).
+  // four, 50 -> 56 us for 16 groups of 4096 rows of 2048 bf16, 151 -> 175 us for 32768 of
+  // 1024, 29 -> 27 us for 20000 rows of 1024 f32, no difference for text).
   const int nv = ve * (b->dtype == Q3S_DTYPE_F32 ? 4 : 2) < 16 ? 8 / ve
                  : b->hidden > 64 * ve                         ? 4
                  : b->hidden > 32 * ve                         ? 2
@@ -937,7 +945,7 @@ int embed_grad(q3s_context* ctx, const q3s_embed_grad_batch* b, void* stream) {
   a.tiles = (b->hidden + tile - 1) / tile;
   // The sort's clusters: as many blocks as leave each 4096 rows, as long as there
   // is a bucket size with which all blocks find a multiprocessor (16 groups of 32768
-  // rows: 162 us, 167 us in single blocks; 16 groups of 4096: 48 us, 54 us with clusters
+  // rows: 151 us, 155 us in single blocks; 16 groups of 4096: 50 us, 55 us with clusters
   // from 1024 rows a block on).
   long long all = 0;
   for (int g = 0; g < groups; ++g) all += a.vocab[g];
@@ -955,12 +963,13 @@ int embed_grad(q3s_context* ctx, const q3s_embed_grad_batch* b, void* stream) {
     ++a.bucket_bits;
   // Codes per warp: as many as leave two warps for every place on the device
   // (32 a multiprocessor).  One code a warp: 16384 rows into 100003 codes 84 -> 90 us, 16
-  // groups of 4096 48 -> 70 us; an eighth of the warps: 100 and 58 us.
+  // groups of 4096 50 -> 71 us; an eighth of the warps: 102 and 59 us.
   const long long units = all * a.tiles;
   const long long chunk = units / (2LL * 32 * ci.sm_count);
   a.chunk = chunk < 1 ? 1 : chunk > 32 ? 32 : (int)chunk;
-  // ... but not so many that the rows of a warp, on average, exceed 64 (16 groups of
-  // 32768 rows: 162 us, 164 us without this).
+  // ... but not so many that the rows of a warp, on average, exceed 64: a bound on what
+  // one warp still has to do when the others are done (16 groups of 32768 rows 151 us
+  // with and without it).
   while (a.chunk > 1 && a.chunk * b->num_rows > 64LL * max_vocab) a.chunk /= 2;
   a.blocks = b->num_rows > 2 * a.block ? (int)((b->num_rows + a.block - 1) / a.block) : 0;
   a.slots = a.blocks * 2 * a.tiles;

@@ -12,12 +12,12 @@
 // a chunk of one row: it asks for the entries that the mask allows, counts the
 // row's history ids that fall into the chunk in shared memory while they are on
 // their way (integer atomics, so the order does not matter), and makes one pass
-// over them.  The entries of the bias list, which are few, are written by one
-// warp at the end.  In place, entries that nothing changes are neither read nor
+// over them.  The entries of the bias list, which are few as a rule, are written by
+// one warp at the end.  In place, entries that nothing changes are neither read nor
 // written.  Latency bounds it: a launch, then metadata, ids, counters, entries.
-// One row of 3072 f32 (256 ids, 8 biases, a mask): 4.1 us; 1024 rows (up to 4096
-// ids, 32 biases, masks): 12.6 us with the rows in L2 (4.5 us at the copy rate), of
-// which 6.3 us without the histories; 48 rows of 100003 bf16 (up to 6000 ids): 16 us.
+// One row of 3072 f32 (256 ids, 8 biases, a mask): 4.0 us; 1024 rows (up to 4096
+// ids, 32 biases, masks): 12.4 us with the rows in L2 (4.5 us at the copy rate), of
+// which 6.8 us without the histories; 48 rows of 100003 bf16 (up to 6000 ids): 15.5 us.
 //
 // stream_kernel, eight rows a multiprocessor or more, of one length up to 4096 and
 // on 16 bytes.  Blocks stay and stream rows through shared memory; see there.
@@ -735,12 +735,12 @@ __device__ __forceinline__ void add_long_lists(const LogitsArgs& a, uint32_t* co
 // for each of them costs less than a look at every counter.
 //
 // HBM bounds it.  61440 rows of 2048, bf16 to f32, with masks and 4 biases (756 MB):
-// 123 us, 94 % of the rate of a copy; 65536 rows of 3072 f32 with 256 ids each
+// 124 us, 93 % of the rate of a copy; 65536 rows of 3072 f32 with 256 ids each
 // (1.6 GB): 272 us, 91 %, the scattered second stores on top.  logits_kernel on the
-// same rows: 263 and 389 us.  One bulk copy a row by one thread: 137 / 327 us where
-// cp.async by all lanes took 157 / 434; with the ids and biases asked for at the
-// top and counted after the row is out, 129 / 308.  T = 64: 32 threads 137 / 371, 128
-// threads 160 / 319.
+// same rows: 238 and 352 us.  Earlier steps: one bulk copy a row by one thread 137 / 327
+// us where cp.async by all lanes took 157 / 434; with the ids and biases asked for at
+// the top and counted after the row is out, 129 / 308; T = 64 then, 32 threads 137 / 371,
+// 128 threads 160 / 319.
 template <int IN, int OUT, int VE, int ROWS, int T>
 __global__ void __launch_bounds__(T, ROWS == 2 ? 6 : 12) stream_kernel(
     const __grid_constant__ LogitsArgs a) {
@@ -930,10 +930,10 @@ cudaError_t launch(LogitsArgs& a, bool aligned, const ContextInfo& ci, cudaStrea
     return (long long)ci.sm_count * (fit < BLOCKS ? fit : BLOCKS);
   };
   // The smallest chunk with which all blocks are on the device at once: few rows
-  // are spread over more blocks (one row of 3072: 4.1 us in three chunks, 6.0 us in
+  // are spread over more blocks (one row of 3072: 4.0 us in three chunks, 6.0 us in
   // one), and long rows, whose every chunk looks at all of the row's history, over
-  // no more than are at work together (48 rows of 100003: 16.6 us with chunks of
-  // 5120, 20.4 us with 3072).  Where none does that, 3072 (600 rows of 30001 f32:
+  // no more than are at work together (48 rows of 100003: 15.5 us with chunks of
+  // 5120, 20.4 us with 3072 at an earlier step).  Where none does that, 3072 (600 rows of 30001 f32:
   // 44 us, 63 us with 8192).
   a.chunk = STEP;
   while (a.chunk <= MAX_CHUNK && a.b.num_rows > held(a.chunk) / chunks(a.chunk)) a.chunk += STEP;
@@ -988,7 +988,7 @@ cudaError_t launch_typed(LogitsArgs& a, const ContextInfo& ci, cudaStream_t st) 
   // Eight rows a multiprocessor, of one length, that start on 16 bytes.  Two rows of
   // 8192 bytes or more in the ring (registers for six blocks a multiprocessor at
   // least; twelve spill, 442 us against 308 for 65536 rows of 3072 f32 at that step),
-  // four of shorter ones (twelve blocks: 123 us for 61440 rows of 2048 bf16, 128 us
+  // four of shorter ones (twelve blocks: 124 us for 61440 rows of 2048 bf16, 128 us
   // with ten).
   const int stage = b.vocab * width<IN>;
   if (b.num_rows >= 8LL * ci.sm_count && !b.row_offsets && !b.row_vocab && !a.in_place && alike &&

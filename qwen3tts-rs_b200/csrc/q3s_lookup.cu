@@ -2,9 +2,9 @@
 // out[i] = scale * table[ids[i]], the f32 product rounded once.
 //
 // HBM-bound gather: a row is read (from L2 where ids repeat) and written once.
-// 65536 ids into 100003 rows of 1024 bf16, a few ids frequent: 38.5 us, 83 % of the
+// 65536 ids into 100003 rows of 1024 bf16, a few ids frequent: 38.4 us, 83 % of the
 // copy rate for each table row read once and the output (32 us); 20011 ids into rows
-// of 1003 f32, which lie on no vector: 27.6 us (20 us).  16 ids of a decode step: 2.9 us,
+// of 1003 f32, which lie on no vector: 27.7 us (20 us).  16 ids of a decode step: 2.9 us,
 // the launch and two accesses one after the other.
 #include <cstdint>
 #include <string>

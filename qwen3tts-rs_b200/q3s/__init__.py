@@ -1045,6 +1045,8 @@ def sample_commit(logits, params, seeds, subseqs, *, codes=None, group: int = 0,
 # `stream` is a raw stream handle (None: torch's current stream).  Outputs that
 # a call makes itself belong to the stream it launches on; inputs used on a
 # stream other than their own must be kept alive and ordered by the caller.
+# int16 ids are the bits of uint16 ones, as in the sampler's histories: -1 is
+# id 65535.  int32 ids below zero are ids from 2^31 on.
 # ---------------------------------------------------------------------------
 _float_types: dict = {}  # torch dtype -> DTYPE_*
 _ids_types: dict = {}    # torch dtype -> IDS_*
@@ -1280,7 +1282,8 @@ def process_logits(logits, *, penalties=None, history=None, history_offsets=None
                    row_vocab=None, vocab: Optional[int] = None, out_dtype=None, out=None,
                    ctx: Optional[Context] = None, stream=None):
     """Penalties for repeated tokens, biases and grammar masks on rows of
-    logits, one launch (q3s_process_logits); the result feeds sample_batch.
+    logits, one launch (q3s_process_logits); the result feeds sample_batch,
+    which takes rows of up to MAX_VOCAB entries, or a sampler of the caller's.
 
     logits: CUDA tensor, float32 or bfloat16, [R, V] (any row stride), or 1-D
     with row_offsets int64 [R], row_vocab int32 [R] and their bound vocab.

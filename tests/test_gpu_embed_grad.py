@@ -510,7 +510,7 @@ def test_workspaces_of_destroyed_graphs_are_used_again():
         del g, out
         gc.collect()
         torch.cuda.synchronize()
-        time.sleep(0.1)  # what a graph holds may be let go on a thread of the driver's
+        time.sleep(0.1)  # what a graph holds may be let go on a thread of CUDA's
     # One workspace is tens of MB; six graphs one after another have one between them.
     assert free[1] - free[-1] < 8 << 20
     ctx.close()
