@@ -439,8 +439,8 @@ __device__ __forceinline__ void add_biases(const Row& row, uint32_t* count, int 
 // stream_kernel, its loop spilled: 61440 rows of 2048 bf16 164 us instead of 126.)
 template <int IN, int OUT, int VE>
 __device__ __forceinline__ void add_many_biases(const LogitsArgs& a, long long r, int part,
-                                             uint32_t* count, Biases& list, char* stage,
-                                             int stage_bytes) {
+                                                uint32_t* count, Biases& list, char* stage,
+                                                int stage_bytes) {
   constexpr int AHEAD = 4;
   constexpr uint32_t NONE = 0xFFFFFFFFu;  // a NaN that no sum is left as
   const int lane = threadIdx.x % 32;
@@ -706,7 +706,7 @@ __global__ void __launch_bounds__(THREADS, BLOCKS) logits_kernel(
 // registers to spare; until then the row's status is that it has not run.
 template <int IN, int OUT, int VE, int T>
 __device__ __forceinline__ void add_long_lists(const LogitsArgs& a, uint32_t* count, Biases& biases,
-                                            char* ring, int ring_bytes) {
+                                               char* ring, int ring_bytes) {
   const int rank = threadIdx.x;
 #pragma unroll 1
   for (long long r = blockIdx.x; r < a.b.num_rows; r += gridDim.x) {
